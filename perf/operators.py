@@ -310,29 +310,29 @@ def _run_own(s):
         if s["mtile_group"] is not None:
             out["mtile_group"] = s["mtile_group"]
         if case["codes"]:
-            moe.gather_i8_device(s["x"], s["row_of_slot"], s["codes"], s["scales"], tokens, top_k, width,
+            moe.gather_i8_device(s["x"], s["row_of_slot"], s["codes"], s["scales"], tokens, top_k, width, s["cap"],
                                  ld_bytes=s["codes"].shape[1], stream=st)
             out.update(codes=s["codes"], scales=s["scales"])
         else:
-            moe.gather_bf16_device(s["x"], s["row_of_slot"], s["gathered"], tokens, top_k, width, stream=st)
+            moe.gather_bf16_device(s["x"], s["row_of_slot"], s["gathered"], tokens, top_k, width, s["cap"], stream=st)
             out["gathered"] = s["gathered"]
-        moe.combine_device(s["out"], s["row_of_slot"], s["weights"], s["y"], tokens, top_k, width, stream=st)
+        moe.combine_device(s["out"], s["row_of_slot"], s["weights"], s["y"], tokens, top_k, width, s["cap"], stream=st)
         out["y"] = s["y"]
         if case["grad"]:
             moe.combine_backward_device(s["grad_y"], s["out"], s["row_of_slot"], s["weights"], s["grad_out"],
-                                        s["grad_weights"], tokens, top_k, width, stream=st)
+                                        s["grad_weights"], tokens, top_k, width, s["cap"], stream=st)
             out.update(grad_out=s["grad_out"], grad_weights=s["grad_weights"])
         return out
     tokens, experts, top_k = case["tokens"], case["experts"], case["top_k"]
     width, hidden, cap = case["width"], case["hidden"], s["out"].shape[0]
     moe.route_device(s["logits"], s["ids"], s["weights"], tokens, experts, top_k, flags=smb.capi.ROUTE_RENORM, stream=st)
     moe.dispatch_device(s["ids"], s["offsets"], s["row_of_slot"], s["slot_of_row"], tokens, top_k, experts, cap, stream=st)
-    moe.gather_i8_device(s["x"], s["row_of_slot"], s["a1"], s["sa1"], tokens, top_k, width, ld_bytes=s["a1"].shape[1],
-                         stream=st)
+    moe.gather_i8_device(s["x"], s["row_of_slot"], s["a1"], s["sa1"], tokens, top_k, width, cap,
+                         ld_bytes=s["a1"].shape[1], stream=st)
     s["plan1"].run(st)
     smb.gemm.quantize_i8_bf16_device(s["h"], s["a2"], s["sa2"], cap, hidden, ld_bytes=s["a2"].shape[1], stream=st)
     s["plan2"].run(st)
-    moe.combine_device(s["out"], s["row_of_slot"], s["weights"], s["y"], tokens, top_k, width, stream=st)
+    moe.combine_device(s["out"], s["row_of_slot"], s["weights"], s["y"], tokens, top_k, width, cap, stream=st)
     return dict(ids=s["ids"], weights=s["weights"], y=s["y"])
 
 
