@@ -428,6 +428,125 @@ int smb_allgather_columns_multi(smb_comm* const* comms, int ndev, const void* co
 int smb_bf16_host_ctx_create_sharded(smb_bf16_host_ctx** ctx, int M, int n_local, int K, smb_comm* comm);
 int smb_fp4_host_ctx_create_sharded(smb_fp4_host_ctx** ctx, int M, int n_local, int K, smb_comm* comm);
 
+/* ------------------------------------------------------------------------------------
+ * int8 GEMM with one scale per token and channel:
+ *   D[m,n] = bf16_rne( (float(sum_k A[m,k] B[n,k]) * sa[m]) * sb[n] ),  the sum exact in int32.
+ * A [M,K] and B [N,K] are int8, row-major, row pitches multiples of 16 bytes, base pointers 16-byte
+ * aligned; sa [M] and sb [N] are fp32; D is bf16 row-major with the store rules of the BF16 GEMM.
+ * Any M, N >= 1 and 1 <= K <= 131071 (the int32 sum of 131072 products could wrap).  No reference
+ * counterpart: its int8 path is not part of the dense GEMM tree.
+ * ---------------------------------------------------------------------------------- */
+
+/* Per-row quantiser, for activations (rows are tokens) and weights (rows are output channels):
+ *   amax = max(max|x|, 2^-100), scale = amax / 127, code = round_half_even(x * (127 / amax)),
+ * every operation in fp32, so all forms agree bit for bit.  A row that holds an infinity or a NaN
+ * gets codes 0 and scale NaN.  K codes per row are written, the rest of the pitch is left alone. */
+int smb_quantize_i8_device(const float* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
+                           int64_t rows, int64_t K, void* stream);
+int smb_quantize_i8_bf16_device(const uint16_t* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes,
+                                float* scales, int64_t rows, int64_t K, void* stream);
+int smb_quantize_i8_host(const float* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
+                         int64_t rows, int64_t K);
+
+/* Plans as for the BF16 GEMM.  Flags: SMB_FLAG_FORCE_PLAIN_STORE, _TILE_N_128 / _256 / _512,
+ * _NO_DECODE, _EPILOGUE_SWIGLU (rows of B interleaved, even = up, odd = gate, D [M, N / 2] =
+ * bf16(silu(gate) * up) of the scaled sums, silu accurate to fp32), _WEIGHTS_STATIC; others are
+ * refused. */
+typedef struct smb_i8_plan smb_i8_plan;
+int smb_i8_plan_create(smb_i8_plan** plan, const void* a, const float* sa, const void* b, const float* sb,
+                       void* d, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldd, unsigned flags);
+/* Fed with BF16 activations [M, K] (row pitch ldx elements, any 2-byte alignment): the plan owns codes
+ * and scales of A and every run quantises `x_bf16` into them first (the rule above).  Such a plan must
+ * not run on two streams at once, nor in two CUDA graphs that may overlap. */
+int smb_i8_plan_create_bf16_activations(smb_i8_plan** plan, const void* x_bf16, int64_t ldx, const void* b,
+                                        const float* sb, void* d, int M, int N, int K, int64_t ldb,
+                                        int64_t ldd, unsigned flags);
+/* Grouped (mixture-of-experts) form with the row offsets in DEVICE memory, as smb_moe_dispatch_device
+ * leaves them: group g owns rows [offsets[g], offsets[g + 1]) of A, sa and D and the N rows
+ * [g N, (g + 1) N) of B and sb.  `offsets` (groups + 1 ints, not decreasing) is read by every run, so
+ * one plan, captured once, serves every batch; max_rows bounds offsets[groups] (rows beyond it are
+ * ignored) and sizes A, sa and D.  Rows outside the groups are not written.  At most 512 groups and
+ * 2^23 rows. */
+int smb_i8_grouped_plan_create(smb_i8_plan** plan, const void* a, const float* sa, const void* b_stacked,
+                               const float* sb_stacked, void* d, int max_rows, int N, int K, int64_t lda,
+                               int64_t ldb, int64_t ldd, int groups, const int* group_offsets_dev,
+                               unsigned flags);
+int smb_i8_plan_run(smb_i8_plan* plan, void* stream);
+int smb_i8_plan_check(smb_i8_plan* plan, void* stream);
+int smb_i8_plan_destroy(smb_i8_plan* plan);
+int smb_i8_plan_describe(smb_i8_plan* plan, char* out, size_t capacity);
+int smb_i8_plan_wait_probe(smb_i8_plan* plan, long long budget_cycles, void* stream);
+int smb_i8_plan_tune(smb_i8_plan* plan, int group_m, int max_clusters);
+/* One-shot on device pointers (lda = ldb = K, so K % 16 == 0) and on host buffers (any K). */
+int smb_dense_gemm_i8(const void* a, const float* sa, const void* b, const float* sb, void* d, int M, int N,
+                      int K, void* stream);
+int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, const float* sb, uint16_t* d,
+                           int M, int N, int K);
+
+/* ------------------------------------------------------------------------------------
+ * Routing to experts and the rows of the grouped GEMMs.  All on the device, stream-ordered, without
+ * host synchronisation, atomics or allocation: a whole expert layer can be captured in a CUDA graph.
+ * tokens == 0 is a valid, empty call (pointers to its empty arrays may be NULL).  No reference counterpart (its tree has the tile map of a
+ * grouped GEMM only, composites/83_grouped_gemm_tile_map.cuh:71-101).
+ * ---------------------------------------------------------------------------------- */
+#define SMB_DTYPE_F32 0
+#define SMB_DTYPE_BF16 1
+#define SMB_ROUTE_SOFTMAX 0u      /* p = softmax over the experts (default) */
+#define SMB_ROUTE_SIGMOID 1u      /* p = 1 / (1 + exp(-logit)) */
+#define SMB_ROUTE_RENORM 2u       /* weights divided by the sum of the chosen p */
+#define SMB_ROUTE_GROUP_TOP2 4u   /* a group is valued by the sum of its two best scores, else by its best */
+/* logits [tokens, experts] (fp32 or bf16, pitch ld) -> ids [tokens, top_k] and weights [tokens, top_k],
+ * best expert first, ties to the lowest index.  Compared are p + bias (bias: [experts] fp32 or NULL; it
+ * takes no part in the weights), without a bias the logits.  With top_groups < n_groups only experts of
+ * the top_groups best of n_groups equal runs of experts can be chosen.  weight = scale * p, or with
+ * RENORM scale * p / sum.  Experts whose logit is -inf or NaN (or bias -inf) are closed; where fewer
+ * than top_k are open the remaining slots hold id -1 and weight 0 (so a padding row of -inf routes
+ * nowhere).  Up to 512 experts, top_k <= 32, n_groups <= 32. */
+int smb_moe_route_device(const void* logits, int dtype, int64_t ld, const float* bias, int tokens, int experts,
+                         int top_k, int n_groups, int top_groups, unsigned flags, float scale, int32_t* ids,
+                         float* weights, void* stream);
+/* Gradient of the logits for the ids that the forward pass chose (the choice itself has none):
+ * grad_weights [tokens, top_k] -> grad_logits [tokens, experts] in the logits' type, all of it written. */
+int smb_moe_route_backward_device(const void* logits, int dtype, int64_t ld, const int32_t* ids,
+                                  const float* grad_weights, int tokens, int experts, int top_k,
+                                  unsigned flags, float scale, void* grad_logits, int64_t ld_grad,
+                                  void* stream);
+
+/* Rows the sorted buffer must have room for: tokens * top_k, plus the padding where align > 1. */
+int64_t smb_moe_max_rows(int64_t tokens, int top_k, int groups, int align);
+/* ids [tokens, top_k] -> layout of the rows sorted by group (stable: slots keep their order):
+ *   offsets [groups + 1]        first row of every group, each a multiple of `align`
+ *   row_of_slot [tokens, top_k] row of every slot; -1 where the id is outside [0, groups)
+ *   slot_of_row [max_rows]      slot of every row, -1 for padding
+ *   mtile_group [max_rows / 256] or NULL: the map of smb_bf16_grouped_plan_create (align % 256 == 0);
+ *                               tiles behind the last row name the last group
+ * max_rows >= smb_moe_max_rows(...).  align: 1 for the int8 grouped plan, 256 for the BF16 one. */
+int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int top_k, int groups, int align,
+                            int64_t max_rows, int32_t* offsets, int32_t* row_of_slot, int32_t* slot_of_row,
+                            int32_t* mtile_group, void* stream);
+/* Row row_of_slot[t, j] of the output becomes row t of x, as bf16 or quantised (rule of
+ * smb_quantize_i8_bf16_device, quantised once per token).  Rows that no slot names are left alone;
+ * entries outside [0, max_rows) are skipped.  The gradient of x is smb_moe_combine_device without
+ * weights. */
+int smb_moe_gather_bf16_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens,
+                               int top_k, int width, int64_t max_rows, uint16_t* out, int64_t ld_out,
+                               void* stream);
+int smb_moe_gather_i8_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens,
+                             int top_k, int width, int64_t max_rows, int8_t* codes, int64_t ld_bytes,
+                             float* scales, void* stream);
+/* y[t] = bf16( sum_j weights[t, j] * rows[row_of_slot[t, j]] ), fp32 in slot order; weights NULL: all 1;
+ * a token without rows gets zeros. */
+int smb_moe_combine_device(const uint16_t* rows, int64_t ld_rows, const int32_t* row_of_slot,
+                           const float* weights, int64_t tokens, int top_k, int width, int64_t max_rows,
+                           uint16_t* y, int64_t ld_y, void* stream);
+/* grad_rows[row_of_slot[t, j]] = bf16(weights[t, j] * grad_y[t]) and, unless NULL, grad_weights[t, j] =
+ * <grad_y[t], rows[row_of_slot[t, j]]> (0 for slots without a row). */
+int smb_moe_combine_backward_device(const uint16_t* grad_y, int64_t ld_grad_y, const uint16_t* rows,
+                                    int64_t ld_rows, const int32_t* row_of_slot, const float* weights,
+                                    int64_t tokens, int top_k, int width, int64_t max_rows,
+                                    uint16_t* grad_rows, int64_t ld_grad_rows, float* grad_weights,
+                                    void* stream);
+
 #define SMB_FLAG_NONE 0u
 #define SMB_FLAG_FORCE_PLAIN_STORE 1u /* use the non-TMA epilogue even when D is aligned */
 #define SMB_FLAG_TILE_N_128 2u        /* force 256 x 128 tiles */
@@ -484,6 +603,10 @@ int smb_fp4_host_ctx_create_sharded(smb_fp4_host_ctx** ctx, int M, int n_local, 
 #define SMB_FLAG_ACT_QUANT_PER_CTA 32768u
 #define SMB_FLAG_ACT_QUANT_CHAINED 65536u
 #define SMB_FLAG_ACT_QUANT_SHARED 131072u
+/* int8 plans: the caller vouches that B and sb are not written by any work that may still be running
+ * on the stream when a run starts; the kernel then begins to read them before the previous kernel
+ * (the one that makes the activations) has completed. */
+#define SMB_FLAG_WEIGHTS_STATIC 1048576u
 
 #ifdef __cplusplus
 }

@@ -41,6 +41,14 @@ FLAG_ACT_QUANT_CHAINED = 65536
 FLAG_ACT_QUANT_SHARED = 131072
 FLAG_TILE_N_192 = 262144
 FLAG_STREAM_K = 524288
+FLAG_WEIGHTS_STATIC = 1048576
+
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+ROUTE_SOFTMAX = 0
+ROUTE_SIGMOID = 1
+ROUTE_RENORM = 2
+ROUTE_GROUP_TOP2 = 4
 
 _vp = C.c_void_p
 _i = C.c_int
@@ -133,6 +141,34 @@ DECLARED = [
     ("smb_allgather_columns", _i, [_vp, _vp, _vp, _vp, _i, _i, _i64, _vp]),
     ("smb_allgather_columns_multi", _i,
      [C.POINTER(_vp), _i, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_vp), _i, _i, _i64, C.POINTER(_vp)]),
+    ("smb_quantize_i8_device", _i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    ("smb_quantize_i8_bf16_device", _i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp]),
+    ("smb_quantize_i8_host", _i, [_vp, _i64, _vp, _i64, _vp, _i64, _i64]),
+    ("smb_i8_plan_create", _i,
+     [C.POINTER(_vp), _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, C.c_uint]),
+    ("smb_i8_plan_create_bf16_activations", _i,
+     [C.POINTER(_vp), _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, C.c_uint]),
+    ("smb_i8_grouped_plan_create", _i,
+     [C.POINTER(_vp), _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i64, _i64, _i64, _i, _vp, C.c_uint]),
+    ("smb_i8_plan_run", _i, [_vp, _vp]),
+    ("smb_i8_plan_check", _i, [_vp, _vp]),
+    ("smb_i8_plan_destroy", _i, [_vp]),
+    ("smb_i8_plan_describe", _i, [_vp, C.c_char_p, C.c_size_t]),
+    ("smb_i8_plan_wait_probe", _i, [_vp, C.c_longlong, _vp]),
+    ("smb_i8_plan_tune", _i, [_vp, _i, _i]),
+    ("smb_dense_gemm_i8", _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _vp]),
+    ("smb_dense_gemm_i8_host", _i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i]),
+    ("smb_moe_route_device", _i,
+     [_vp, _i, _i64, _vp, _i, _i, _i, _i, _i, C.c_uint, C.c_float, _vp, _vp, _vp]),
+    ("smb_moe_route_backward_device", _i,
+     [_vp, _i, _i64, _vp, _vp, _i, _i, _i, C.c_uint, C.c_float, _vp, _i64, _vp]),
+    ("smb_moe_max_rows", _i64, [_i64, _i, _i, _i]),
+    ("smb_moe_dispatch_device", _i, [_vp, _i64, _i, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp]),
+    ("smb_moe_gather_bf16_device", _i, [_vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp]),
+    ("smb_moe_gather_i8_device", _i, [_vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp, _vp]),
+    ("smb_moe_combine_device", _i, [_vp, _i64, _vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp]),
+    ("smb_moe_combine_backward_device", _i,
+     [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp, _vp]),
 ]
 
 PEER_HANDLE_BYTES = 64

@@ -1,0 +1,521 @@
+// Rows to experts and back: the layout the grouped GEMMs read, and the weighted sum of what they write.
+//
+//   dispatch   ids [tokens, top_k] -> a stable counting sort of the slots by expert: row offsets of the
+//              experts, slot -> row and row -> slot maps
+//   gather     row_of_slot[t, j] = r: row r of the sorted buffer becomes row t of x (bf16, or int8 codes
+//              with the row's scale)
+//   combine    y[t] = sum_j weights[t, j] * rows[row_of_slot[t, j]], and its gradients
+//
+// A slot that goes nowhere (id outside [0, experts)) has row -1 and is skipped everywhere; rows that no
+// slot names are never written.  No atomics: the order of every sum and of the rows is fixed.
+#include <cooperative_groups.h>
+
+#include "i8_common.cuh"
+#include "ptx.cuh"
+#include "quant_i8.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace smb {
+namespace {
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kMaxDispatchGroups = 1024;
+constexpr int kMaxTopKRows = 32;
+
+cudaLaunchConfig_t pdl_config(dim3 grid, dim3 block, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// --------------------------------------------------------------------------- dispatch
+struct DispatchParams {
+  const int* ids;
+  int n;               // slots
+  int groups, align;
+  int cap;             // rows of the sorted buffer
+  int per_warp;        // slots per warp, a multiple of 32
+  int* offsets;
+  int* row_of_slot;
+  int* slot_of_row;
+  int* mtile_group;
+};
+
+// One cluster sorts everything: warp w of the cluster owns the slots [w * per_warp, + per_warp), so
+// "earlier slots" means earlier lanes, earlier chunks, earlier warps, earlier CTAs, and the counts of the
+// CTAs meet through distributed shared memory instead of a second launch.
+//   shared: hist[warps][groups] | total[groups] | start[groups] | padded[groups]
+__global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) {
+  extern __shared__ int sm[];
+  cg::cluster_group cluster = cg::this_cluster();
+  griddep_launch_dependents();
+  griddep_wait();
+  const int warps = blockDim.x >> 5;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int G = p.groups;
+  int* hist = sm;
+  int* total = hist + warps * G;
+  int* start = total + G;
+  int* padded = start + G;
+  __shared__ int rows_used;
+
+  for (int i = threadIdx.x; i < warps * G; i += blockDim.x) hist[i] = 0;
+  __syncthreads();
+  int* mine = hist + warp * G;
+  const long long first = static_cast<long long>(rank * warps + warp) * p.per_warp;
+  const int lo = static_cast<int>(first < p.n ? first : p.n);
+  const int hi = static_cast<int>(first + p.per_warp < p.n ? first + p.per_warp : p.n);
+  for (int s0 = lo; s0 < hi; s0 += 32) {
+    const int s = s0 + lane;
+    int e = s < hi ? p.ids[s] : -1;
+    if (e < 0 || e >= G) e = -1;
+    const unsigned same = __match_any_sync(kFull, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < G; e += blockDim.x) {
+    int before = 0;
+    for (int w = 0; w < warps; ++w) {
+      const int c = hist[w * G + e];
+      hist[w * G + e] = before;
+      before += c;
+    }
+    total[e] = before;
+  }
+  cluster.sync();
+  for (int e = threadIdx.x; e < G; e += blockDim.x) {
+    int before = 0, all = 0;
+    for (int c = 0; c < ctas; ++c) {
+      const int v = *cluster.map_shared_rank(total + e, c);
+      if (c < rank) before += v;
+      all += v;
+    }
+    start[e] = before;
+    padded[e] = all;
+  }
+  cluster.sync();   // also: nobody's shared memory is read by another CTA after this
+  if (warp == 0) {
+    // Exclusive scan of the padded counts: a run of groups per lane, then five shuffles.
+    const int per = (G + 31) / 32;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e < G) sum += (padded[e] + p.align - 1) / p.align * p.align;
+    }
+    int before = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(kFull, before, d);
+      if (lane >= d) before += up;
+    }
+    if (lane == 31) rows_used = before;
+    before -= sum;
+    for (int i = 0; i < per; ++i) {
+      const int e = lane * per + i;
+      if (e < G) {
+        const int size = (padded[e] + p.align - 1) / p.align * p.align;
+        total[e] = before;                  // first row of the group, from here on
+        start[e] += before;
+        if (rank == 0) p.offsets[e] = before;
+        before += size;
+      }
+    }
+    if (rank == 0 && lane == 31) p.offsets[G] = rows_used;
+  }
+  __syncthreads();
+  const int used = rows_used;
+  for (int s0 = lo; s0 < hi; s0 += 32) {
+    const int s = s0 + lane;
+    int e = s < hi ? p.ids[s] : -1;
+    if (e < 0 || e >= G) e = -1;
+    const unsigned same = __match_any_sync(kFull, e);
+    int row = -1;
+    if (e >= 0) row = start[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
+    __syncwarp();
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+    if (s < hi) p.row_of_slot[s] = row;
+    if (row >= 0) p.slot_of_row[row] = s;
+  }
+  // Rows that no slot names: the padding of every group, and everything behind the last one.
+  const int threads = ctas * blockDim.x;
+  const int me = rank * blockDim.x + threadIdx.x;
+  if (p.align > 1) {
+    for (int e = me >> 5; e < G; e += threads >> 5) {
+      const int end = e + 1 < G ? total[e + 1] : used;
+      for (int r = total[e] + padded[e] + lane; r < end; r += 32) p.slot_of_row[r] = -1;
+    }
+  }
+  for (int r = used + me; r < p.cap; r += threads) p.slot_of_row[r] = -1;
+  if (p.mtile_group != nullptr) {
+    for (int e = me >> 5; e < G; e += threads >> 5) {
+      const int end = e + 1 < G ? total[e + 1] : used;
+      for (int t = total[e] / 256 + lane; t < end / 256; t += 32) p.mtile_group[t] = e;
+    }
+    for (int t = used / 256 + me; t < p.cap / 256; t += threads) p.mtile_group[t] = G - 1;
+  }
+}
+
+// --------------------------------------------------------------------------- gather
+constexpr int kCta = 256;
+
+template <bool kAligned>
+__global__ void __launch_bounds__(kCta) gather_bf16_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int top_k,
+                                                           int width, int max_rows, uint16_t* out, int64_t ld_out) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int64_t t = blockIdx.x;
+  const int* rows = row_of_slot + t * top_k;
+  const uint16_t* src = x + t * ld_x;
+  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  if (c0 >= width) return;
+  if (kAligned && c0 + 8 <= width) {
+    const uint4 v = *reinterpret_cast<const uint4*>(src + c0);
+    for (int j = 0; j < top_k; ++j) {
+      const int r = rows[j];
+      if (r >= 0 && r < max_rows) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * ld_out + c0) = v;
+    }
+    return;
+  }
+  const int end = min(c0 + 8, width);
+  for (int j = 0; j < top_k; ++j) {
+    const int r = rows[j];
+    if (r < 0 || r >= max_rows) continue;
+    for (int c = c0; c < end; ++c) out[static_cast<int64_t>(r) * ld_out + c] = src[c];
+  }
+}
+
+template <int kThreads, bool kAligned>
+__global__ void __launch_bounds__(kCta) gather_i8_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot,
+                                                         int64_t tokens, int top_k, int width, int max_rows, int8_t* codes,
+                                                         int64_t ld_bytes, float* scales) {
+  __shared__ uint32_t red[kCta / 32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x % kThreads;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kCta / kThreads) + threadIdx.x / kThreads;
+  if (t >= tokens) return;   // whole warps, and whole CTAs where a row has more than one
+  const int* rows = row_of_slot + t * top_k;
+  const float scale = qi8::quantize_row<true, kThreads, 4, kAligned>(
+      x + t * ld_x, width, tid, red,
+      [&](int k, uint2 c) {
+        for (int j = 0; j < top_k; ++j) {
+          const int r = rows[j];
+          if (r >= 0 && r < max_rows) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * ld_bytes + k) = c;
+        }
+      },
+      [&](int k, int8_t c) {
+        for (int j = 0; j < top_k; ++j) {
+          const int r = rows[j];
+          if (r >= 0 && r < max_rows) codes[static_cast<int64_t>(r) * ld_bytes + k] = c;
+        }
+      });
+  if (tid < top_k) {
+    const int r = rows[tid];
+    if (r >= 0 && r < max_rows) scales[r] = scale;
+  }
+}
+
+// --------------------------------------------------------------------------- combine
+__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ float bf16_one(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
+__device__ __forceinline__ uint16_t to_bf16(float v) {
+  return static_cast<uint16_t>(pack_bf16x2(__float_as_uint(v), 0u) & 0xFFFFu);
+}
+
+// fp32 sum in slot order, one rounding to bf16.
+template <bool kAligned>
+__global__ void __launch_bounds__(kCta) combine_kernel(const uint16_t* rows_in, int64_t ld_rows, const int* row_of_slot,
+                                                       const float* weights, int top_k, int width, int max_rows, uint16_t* y,
+                                                       int64_t ld_y) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int64_t t = blockIdx.x;
+  const int* rows = row_of_slot + t * top_k;
+  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  if (c0 >= width) return;
+  float acc[8] = {};
+  const int n = min(8, width - c0);
+  const bool whole = kAligned && n == 8;
+#pragma unroll 4
+  for (int j = 0; j < top_k; ++j) {
+    const int r = rows[j];
+    if (r < 0 || r >= max_rows) continue;
+    const float w = weights != nullptr ? weights[t * top_k + j] : 1.0f;
+    const uint16_t* src = rows_in + static_cast<int64_t>(r) * ld_rows + c0;
+    if (whole) {
+      const uint4 q = *reinterpret_cast<const uint4*>(src);
+      const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[2 * i] = fmaf(w, bf16_lo(v[i]), acc[2 * i]);
+        acc[2 * i + 1] = fmaf(w, bf16_hi(v[i]), acc[2 * i + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) acc[i] = fmaf(w, bf16_one(src[i]), acc[i]);
+    }
+  }
+  uint16_t* dst = y + t * ld_y + c0;
+  if (whole) {
+    uint4 q;
+    q.x = pack_bf16x2(__float_as_uint(acc[0]), __float_as_uint(acc[1]));
+    q.y = pack_bf16x2(__float_as_uint(acc[2]), __float_as_uint(acc[3]));
+    q.z = pack_bf16x2(__float_as_uint(acc[4]), __float_as_uint(acc[5]));
+    q.w = pack_bf16x2(__float_as_uint(acc[6]), __float_as_uint(acc[7]));
+    *reinterpret_cast<uint4*>(dst) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) dst[i] = to_bf16(acc[i]);
+  }
+}
+
+// A warp per slot: its row's gradient w * dy and its weight's gradient <dy, row>.  The warps of a token
+// are neighbours, so dy comes from L1 after the first of them.
+template <bool kAligned>
+__global__ void __launch_bounds__(kCta) combine_grad_kernel(const uint16_t* grad_y, int64_t ld_gy, const uint16_t* rows_in,
+                                                            int64_t ld_rows, const int* row_of_slot, const float* weights,
+                                                            int64_t slots, int top_k, int width, int max_rows,
+                                                            uint16_t* grad_rows, int64_t ld_gr, float* grad_weights) {
+  griddep_launch_dependents();
+  griddep_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t s = static_cast<int64_t>(blockIdx.x) * (kCta / 32) + (threadIdx.x >> 5);
+  if (s >= slots) return;
+  const int r = row_of_slot[s];
+  if (r < 0 || r >= max_rows) {
+    if (lane == 0 && grad_weights != nullptr) grad_weights[s] = 0.0f;
+    return;
+  }
+  const float w = weights != nullptr ? weights[s] : 1.0f;
+  const uint16_t* gy = grad_y + s / top_k * ld_gy;
+  const uint16_t* in = rows_in != nullptr ? rows_in + static_cast<int64_t>(r) * ld_rows : nullptr;
+  uint16_t* out = grad_rows + static_cast<int64_t>(r) * ld_gr;
+  float dot = 0.0f;
+  const int whole = kAligned ? width / 8 * 8 : 0;
+  for (int c = lane * 8; c < whole; c += 256) {
+    const uint4 g4 = *reinterpret_cast<const uint4*>(gy + c);
+    const uint32_t g[4] = {g4.x, g4.y, g4.z, g4.w};
+    if (grad_weights != nullptr) {
+      const uint4 v4 = *reinterpret_cast<const uint4*>(in + c);
+      const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dot = fmaf(bf16_lo(g[i]), bf16_lo(v[i]), dot);
+        dot = fmaf(bf16_hi(g[i]), bf16_hi(v[i]), dot);
+      }
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = pack_bf16x2(__float_as_uint(w * bf16_lo(g[i])), __float_as_uint(w * bf16_hi(g[i])));
+    *reinterpret_cast<uint4*>(out + c) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+  for (int c = whole + lane; c < width; c += 32) {
+    const float g = bf16_one(gy[c]);
+    if (grad_weights != nullptr) dot = fmaf(g, bf16_one(in[c]), dot);
+    out[c] = to_bf16(w * g);
+  }
+  if (grad_weights != nullptr) {
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(kFull, dot, d);
+    if (lane == 0) grad_weights[s] = dot;
+  }
+}
+
+bool aligned16(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
+bool aligned_to(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int finish(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? SMB_OK : set_cuda_error(e, what);
+}
+
+// What the row copies and sums share.
+int check_rows(const char* what, const void* row_of_slot, int64_t tokens, int top_k, int width, int64_t max_rows) {
+  if (tokens != 0 && row_of_slot == nullptr) return set_error(SMB_ERR_INVALID, "%s: null row map", what);
+  if (!aligned_to(row_of_slot, 4)) return set_error(SMB_ERR_INVALID, "%s: row map is not 4-byte aligned", what);
+  if (tokens < 0 || tokens > 0x7FFFFFFFLL) return set_error(SMB_ERR_INVALID, "%s: bad token count", what);
+  if (top_k < 1 || top_k > kMaxTopKRows)
+    return set_error(SMB_ERR_INVALID, "%s: top_k=%d outside 1..%d", what, top_k, kMaxTopKRows);
+  if (width < 1 || width > 65535 * 8 * 32) return set_error(SMB_ERR_INVALID, "%s: width %d out of range", what, width);
+  if (max_rows < (tokens != 0 ? 1 : 0) || max_rows > 0x7FFFFFFFLL)
+    return set_error(SMB_ERR_INVALID, "%s: bad row capacity", what);
+  return SMB_OK;
+}
+
+// Threads for a row in vectors of eight: whole warps, at most a CTA; the rest goes to the grid's y.
+void row_grid(int64_t tokens, int width, dim3* grid, dim3* block) {
+  const int vecs = (width + 7) / 8;
+  int threads = (vecs + 31) / 32 * 32;
+  if (threads > 128) threads = 128;
+  *block = dim3(static_cast<unsigned>(threads), 1, 1);
+  *grid = dim3(static_cast<unsigned>(tokens), static_cast<unsigned>((vecs + threads - 1) / threads), 1);
+}
+
+}  // namespace
+}  // namespace smb
+
+using namespace smb;
+
+extern "C" int64_t smb_moe_max_rows(int64_t tokens, int top_k, int groups, int align) {
+  if (tokens < 0 || top_k < 1 || groups < 1 || align < 1) return 0;
+  const int64_t n = tokens * top_k;
+  const int64_t hit = groups < n ? groups : n;
+  return (n + hit * (align - 1)) / align * align;
+}
+
+extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int top_k, int groups, int align, int64_t max_rows,
+                                       int32_t* offsets, int32_t* row_of_slot, int32_t* slot_of_row, int32_t* mtile_group,
+                                       void* stream) {
+  // An empty batch has no ids and no row map, and with align 1 no rows either.
+  if (offsets == nullptr || (tokens != 0 && (ids == nullptr || row_of_slot == nullptr)) ||
+      (max_rows != 0 && slot_of_row == nullptr))
+    return set_error(SMB_ERR_INVALID, "dispatch: null pointer");
+  if (!aligned_to(ids, 4) || !aligned_to(offsets, 4) || !aligned_to(row_of_slot, 4) || !aligned_to(slot_of_row, 4) ||
+      !aligned_to(mtile_group, 4))
+    return set_error(SMB_ERR_INVALID, "dispatch: pointers must be 4-byte aligned");
+  if (groups < 1 || groups > kMaxDispatchGroups)
+    return set_error(SMB_ERR_UNSUPPORTED, "dispatch: %d groups outside 1..%d", groups, kMaxDispatchGroups);
+  if (tokens < 0 || top_k < 1 || top_k > kMaxTopKRows)
+    return set_error(SMB_ERR_INVALID, "dispatch: bad extents (tokens=%lld top_k=%d)", static_cast<long long>(tokens), top_k);
+  if (align < 1 || align > 65536) return set_error(SMB_ERR_INVALID, "dispatch: alignment %d outside 1..65536", align);
+  if (mtile_group != nullptr && align % 256 != 0)
+    return set_error(SMB_ERR_INVALID, "dispatch: the tile map needs groups aligned to 256 rows, not %d", align);
+  if (tokens > (1LL << 30) / top_k) return set_error(SMB_ERR_UNSUPPORTED, "dispatch: more than 2^30 slots");
+  const int64_t need = smb_moe_max_rows(tokens, top_k, groups, align);
+  if (max_rows < need || max_rows > 0x7FFFFFFFLL)
+    return set_error(SMB_ERR_INVALID, "dispatch: room for %lld rows, up to %lld may be needed",
+                     static_cast<long long>(max_rows), static_cast<long long>(need));
+  DispatchParams p = {};
+  p.ids = ids;
+  p.n = static_cast<int>(tokens * top_k);
+  p.groups = groups;
+  p.align = align;
+  p.cap = static_cast<int>(max_rows);
+  p.offsets = offsets;
+  p.row_of_slot = row_of_slot;
+  p.slot_of_row = slot_of_row;
+  p.mtile_group = mtile_group;
+  // Warps: as many as have 32 slots each, up to 32 in a CTA and 8 CTAs; the histograms bound them too.
+  int warps = (p.n + 31) / 32;
+  if (warps < 4) warps = 4;
+  int ctas = 1;
+  while (ctas < 8 && warps > 32 * ctas) ctas *= 2;
+  warps = (warps + ctas - 1) / ctas;
+  if (warps > 32) warps = 32;
+  p.per_warp = static_cast<int>((p.n + static_cast<int64_t>(ctas) * warps * 32 - 1) / (static_cast<int64_t>(ctas) * warps * 32)) * 32;
+  const size_t smem = static_cast<size_t>(warps + 3) * groups * sizeof(int);
+  cudaError_t e = cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       35 * kMaxDispatchGroups * static_cast<int>(sizeof(int)));
+  if (e != cudaSuccess) return set_cuda_error(e, "dispatch shared memory");
+  cudaLaunchAttribute attr[2];
+  cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, 1, 1), dim3(warps * 32, 1, 1), smem, static_cast<cudaStream_t>(stream), attr);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = 2;
+  return finish(cudaLaunchKernelEx(&cfg, dispatch_kernel, p), "dispatch launch");
+}
+
+extern "C" int smb_moe_gather_bf16_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens,
+                                          int top_k, int width, int64_t max_rows, uint16_t* out, int64_t ld_out,
+                                          void* stream) {
+  if (tokens != 0 && (x == nullptr || out == nullptr)) return set_error(SMB_ERR_INVALID, "gather: null pointer");
+  if (int rc = check_rows("gather", row_of_slot, tokens, top_k, width, max_rows)) return rc;
+  if (ld_x < width || ld_out < width) return set_error(SMB_ERR_INVALID, "gather: pitch smaller than the row");
+  if (!aligned_to(x, 2) || !aligned_to(out, 2)) return set_error(SMB_ERR_INVALID, "gather: rows are not 2-byte aligned");
+  if (tokens == 0) return SMB_OK;
+  const bool al = aligned16(x, ld_x * 2) && aligned16(out, ld_out * 2);
+  dim3 grid, block;
+  row_grid(tokens, width, &grid, &block);
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, al ? gather_bf16_kernel<true> : gather_bf16_kernel<false>, x, ld_x, row_of_slot, top_k,
+                                   width, static_cast<int>(max_rows), out, ld_out),
+                "gather launch");
+}
+
+extern "C" int smb_moe_gather_i8_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens, int top_k,
+                                        int width, int64_t max_rows, int8_t* codes, int64_t ld_bytes, float* scales,
+                                        void* stream) {
+  if (tokens != 0 && (x == nullptr || codes == nullptr || scales == nullptr))
+    return set_error(SMB_ERR_INVALID, "i8 gather: null pointer");
+  if (int rc = check_rows("i8 gather", row_of_slot, tokens, top_k, width, max_rows)) return rc;
+  if (ld_x < width || ld_bytes < width) return set_error(SMB_ERR_INVALID, "i8 gather: pitch smaller than the row");
+  if (!aligned_to(x, 2) || !aligned_to(scales, 4))
+    return set_error(SMB_ERR_INVALID, "i8 gather: rows must be 2-byte, scales 4-byte aligned");
+  if (tokens == 0) return SMB_OK;
+  const bool al = aligned16(x, ld_x * 2) && aligned_to(codes, 8) && ld_bytes % 8 == 0;
+  const bool narrow = width <= 1024;   // a warp holds such a row in registers
+  const int64_t per_cta = narrow ? kCta / 32 : 1;
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((tokens + per_cta - 1) / per_cta), 1, 1), dim3(kCta, 1, 1), 0,
+                                      static_cast<cudaStream_t>(stream), &attr);
+  auto kernel = narrow ? (al ? gather_i8_kernel<32, true> : gather_i8_kernel<32, false>)
+                       : (al ? gather_i8_kernel<kCta, true> : gather_i8_kernel<kCta, false>);
+  return finish(cudaLaunchKernelEx(&cfg, kernel, x, ld_x, row_of_slot, tokens, top_k, width, static_cast<int>(max_rows), codes,
+                                   ld_bytes, scales),
+                "i8 gather launch");
+}
+
+extern "C" int smb_moe_combine_device(const uint16_t* rows, int64_t ld_rows, const int32_t* row_of_slot, const float* weights,
+                                      int64_t tokens, int top_k, int width, int64_t max_rows, uint16_t* y, int64_t ld_y,
+                                      void* stream) {
+  if (tokens != 0 && (rows == nullptr || y == nullptr)) return set_error(SMB_ERR_INVALID, "combine: null pointer");
+  if (int rc = check_rows("combine", row_of_slot, tokens, top_k, width, max_rows)) return rc;
+  if (ld_rows < width || ld_y < width) return set_error(SMB_ERR_INVALID, "combine: pitch smaller than the row");
+  if (!aligned_to(rows, 2) || !aligned_to(y, 2) || !aligned_to(weights, 4))
+    return set_error(SMB_ERR_INVALID, "combine: rows must be 2-byte, weights 4-byte aligned");
+  if (tokens == 0) return SMB_OK;
+  const bool al = aligned16(rows, ld_rows * 2) && aligned16(y, ld_y * 2);
+  dim3 grid, block;
+  row_grid(tokens, width, &grid, &block);
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, al ? combine_kernel<true> : combine_kernel<false>, rows, ld_rows, row_of_slot, weights,
+                                   top_k, width, static_cast<int>(max_rows), y, ld_y),
+                "combine launch");
+}
+
+extern "C" int smb_moe_combine_backward_device(const uint16_t* grad_y, int64_t ld_grad_y, const uint16_t* rows,
+                                               int64_t ld_rows, const int32_t* row_of_slot, const float* weights,
+                                               int64_t tokens, int top_k, int width, int64_t max_rows, uint16_t* grad_rows,
+                                               int64_t ld_grad_rows, float* grad_weights, void* stream) {
+  if (tokens != 0 && (grad_y == nullptr || grad_rows == nullptr))
+    return set_error(SMB_ERR_INVALID, "combine backward: null pointer");
+  if (tokens != 0 && grad_weights != nullptr && rows == nullptr)
+    return set_error(SMB_ERR_INVALID, "combine backward: the weights' gradient needs the rows");
+  if (int rc = check_rows("combine backward", row_of_slot, tokens, top_k, width, max_rows)) return rc;
+  if (ld_grad_y < width || ld_grad_rows < width || (rows != nullptr && ld_rows < width))
+    return set_error(SMB_ERR_INVALID, "combine backward: pitch smaller than the row");
+  if (!aligned_to(grad_y, 2) || !aligned_to(rows, 2) || !aligned_to(grad_rows, 2) || !aligned_to(weights, 4) ||
+      !aligned_to(grad_weights, 4))
+    return set_error(SMB_ERR_INVALID, "combine backward: rows must be 2-byte, weights 4-byte aligned");
+  if (tokens == 0) return SMB_OK;
+  const bool al = aligned16(grad_y, ld_grad_y * 2) && aligned16(grad_rows, ld_grad_rows * 2) &&
+                  (rows == nullptr || aligned16(rows, ld_rows * 2));
+  const int64_t slots = tokens * top_k;
+  if ((slots + kCta / 32 - 1) / (kCta / 32) > 0x7FFFFFFFLL) return set_error(SMB_ERR_UNSUPPORTED, "combine backward: too many slots");
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((slots + kCta / 32 - 1) / (kCta / 32)), 1, 1), dim3(kCta, 1, 1),
+                                      0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, al ? combine_grad_kernel<true> : combine_grad_kernel<false>, grad_y, ld_grad_y, rows,
+                                   ld_rows, row_of_slot, weights, slots, top_k, width, static_cast<int>(max_rows), grad_rows,
+                                   ld_grad_rows, grad_weights),
+                "combine backward launch");
+}

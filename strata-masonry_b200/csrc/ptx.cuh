@@ -311,6 +311,13 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16(int mma_m, int mma_n) {
          ((static_cast<uint32_t>(mma_m) >> 4) << 24);
 }
 
+// Instruction descriptor, kind::i8 with signed operands, int32 accumulate, both operands K-major.
+// [4,6) D format (2 = S32); [7,10) A format (1 = signed); [10,13) B format; N and M as above.
+__host__ __device__ constexpr uint32_t make_idesc_i8(int mma_m, int mma_n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((static_cast<uint32_t>(mma_n) >> 3) << 17) |
+         ((static_cast<uint32_t>(mma_m) >> 4) << 24);
+}
+
 // Instruction descriptor, kind::mxf4nvf4 with E2M1 operands, block scales.
 // [4,6) B scale-factor id; [7,10) A format (1 = E2M1); [10,13) B format (1 = E2M1);
 // [17,23) N >> 3; [23] scale type (1 = UE8M0); [27,29) M >> 7; [29,31) A scale-factor id.
@@ -342,6 +349,31 @@ __device__ __forceinline__ void mma_bf16_ss(uint32_t tmem_d, uint64_t desc_a, ui
         ".reg .pred p;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  }
+}
+
+// int8 x int8 -> int32, K = 32 per instruction.
+template <int CTA_GROUP>
+__device__ __forceinline__ void mma_i8_ss(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                          uint32_t accumulate) {
+  if constexpr (CTA_GROUP == 1) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+        "}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t"
         "}"
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
@@ -509,6 +541,13 @@ __device__ __forceinline__ void st_global_v4(void* ptr, uint32_t a, uint32_t b, 
                                              uint32_t d) {
   asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(ptr), "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
+}
+
+// Ordinary (coherent) load of an int that an earlier kernel on the stream may have written.
+__device__ __forceinline__ int ld_global_s32(const int* ptr) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(ptr) : "memory");
+  return v;
 }
 
 // Programmatic dependent launch: let the next grid on the stream start early / wait for the

@@ -1,0 +1,127 @@
+// int8 quantiser, one scale per row: the activations of a token, or the weights of an output channel
+// of the int8 product.  Bound by HBM: bf16 rows move 3 bytes per element.
+#include <cmath>
+#include <cstring>
+
+#include "i8_common.cuh"
+#include "quant_i8.cuh"
+
+namespace smb {
+namespace {
+
+constexpr int kCta = 256;
+
+// kThreads of the CTA's 256 threads share a row.
+template <bool kBf16, int kThreads, int kVecs, bool kAligned>
+__global__ void __launch_bounds__(kCta) quantize_i8_kernel(const void* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes,
+                                                           float* scales, int64_t rows, int K) {
+  __shared__ uint32_t red[kCta / 32];
+  griddep_launch_dependents();
+  griddep_wait();
+  const int tid = threadIdx.x % kThreads;
+  const int64_t r = static_cast<int64_t>(blockIdx.x) * (kCta / kThreads) + threadIdx.x / kThreads;
+  if (r >= rows) return;   // whole warps: rows are shared by CTAs only where kThreads == kCta
+  const void* row = static_cast<const char*>(src) + r * ld_src * (kBf16 ? 2 : 4);
+  int8_t* out = codes + r * ld_bytes;
+  const float scale = qi8::quantize_row<kBf16, kThreads, kVecs, kAligned>(
+      row, K, tid, red, [&](int k, uint2 c) { *reinterpret_cast<uint2*>(out + k) = c; },
+      [&](int k, int8_t c) { out[k] = c; });
+  if (tid == 0) scales[r] = scale;
+}
+
+template <bool kBf16, bool kAligned>
+cudaError_t launch_quantize(const cudaLaunchConfig_t& base, const void* src, int64_t ld_src, int8_t* codes,
+                            int64_t ld_bytes, float* scales, int64_t rows, int K) {
+  cudaLaunchConfig_t cfg = base;
+  // A warp holds 1024 elements of its row in registers; longer rows take a whole CTA.
+  if (K <= 1024) {
+    cfg.gridDim = dim3(static_cast<unsigned>((rows + kCta / 32 - 1) / (kCta / 32)), 1, 1);
+    return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, 32, 4, kAligned>, src, ld_src, codes, ld_bytes, scales,
+                              rows, K);
+  }
+  cfg.gridDim = dim3(static_cast<unsigned>(rows), 1, 1);
+  return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, kCta, 4, kAligned>, src, ld_src, codes, ld_bytes, scales,
+                            rows, K);
+}
+
+int check_quantize(const void* src, int64_t ld_src, const void* codes, int64_t ld_bytes, const void* scales, int64_t rows,
+                   int64_t K) {
+  if (rows != 0 && (src == nullptr || codes == nullptr || scales == nullptr))
+    return set_error(SMB_ERR_INVALID, "i8 quantize: null pointer");
+  if (rows < 0 || rows > 0x7FFFFFFFLL || K <= 0 || K > 0x7FFFFFFFLL)
+    return set_error(SMB_ERR_INVALID, "i8 quantize: bad extents (rows=%lld K=%lld)", static_cast<long long>(rows),
+                     static_cast<long long>(K));
+  if (ld_src < K || ld_bytes < K) return set_error(SMB_ERR_INVALID, "i8 quantize: pitch smaller than K");
+  return SMB_OK;
+}
+
+}  // namespace
+
+int quantize_i8_launch(const void* src, bool bf16, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
+                       int64_t rows, int64_t K, cudaStream_t st) {
+  if (rows == 0) return SMB_OK;
+  const int size = bf16 ? 2 : 4;
+  const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0 && (ld_src * size) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ld_bytes % 8 == 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kCta, 1, 1);
+  cfg.stream = st;
+  cudaLaunchAttribute pdl;
+  pdl.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  pdl.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &pdl;
+  cfg.numAttrs = 1;
+  const int k = static_cast<int>(K);
+  cudaError_t e;
+  if (bf16)
+    e = aligned ? launch_quantize<true, true>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
+                : launch_quantize<true, false>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
+  else
+    e = aligned ? launch_quantize<false, true>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
+                : launch_quantize<false, false>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e, "i8 quantize launch");
+  return SMB_OK;
+}
+
+}  // namespace smb
+
+using namespace smb;
+
+extern "C" int smb_quantize_i8_device(const float* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
+                                      int64_t rows, int64_t K, void* stream) {
+  if (int rc = check_quantize(src, ld_src, codes, ld_bytes, scales, rows, K)) return rc;
+  if (reinterpret_cast<uintptr_t>(src) % 4 != 0 || reinterpret_cast<uintptr_t>(scales) % 4 != 0)
+    return set_error(SMB_ERR_INVALID, "i8 quantize: source and scales must be 4-byte aligned");
+  return quantize_i8_launch(src, false, ld_src, codes, ld_bytes, scales, rows, K, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int smb_quantize_i8_bf16_device(const uint16_t* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes,
+                                           float* scales, int64_t rows, int64_t K, void* stream) {
+  if (int rc = check_quantize(src, ld_src, codes, ld_bytes, scales, rows, K)) return rc;
+  if (reinterpret_cast<uintptr_t>(src) % 2 != 0 || reinterpret_cast<uintptr_t>(scales) % 4 != 0)
+    return set_error(SMB_ERR_INVALID, "i8 quantize: source must be 2-byte, scales 4-byte aligned");
+  return quantize_i8_launch(src, true, ld_src, codes, ld_bytes, scales, rows, K, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int smb_quantize_i8_host(const float* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
+                                    int64_t rows, int64_t K) {
+  if (int rc = check_quantize(src, ld_src, codes, ld_bytes, scales, rows, K)) return rc;
+  for (int64_t r = 0; r < rows; ++r) {
+    const float* row = src + r * ld_src;
+    uint32_t m = 0;
+    for (int64_t k = 0; k < K; ++k) {
+      uint32_t bits;
+      memcpy(&bits, row + k, 4);
+      bits &= 0x7FFFFFFFu;
+      m = bits > m ? bits : m;
+    }
+    float amax;
+    memcpy(&amax, &m, 4);
+    const qi8::RowScale rs = qi8::row_scale(amax, m < 0x7F800000u);
+    for (int64_t k = 0; k < K; ++k)
+      codes[r * ld_bytes + k] = rs.bad ? 0 : static_cast<int8_t>(std::nearbyintf(row[k] * rs.inv));
+    scales[r] = rs.bad ? NAN : rs.scale;
+  }
+  return SMB_OK;
+}

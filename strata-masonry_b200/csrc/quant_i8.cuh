@@ -1,0 +1,148 @@
+// Per-row int8 quantiser, shared by the plain quantiser and the one that copies rows to experts.
+//
+//   amax  = max(max_k |x[k]|, 2^-100)           (the floor keeps 127 / amax finite)
+//   scale = fl32(amax / 127),  inv = fl32(127 / amax)
+//   code  = round_half_even(fl32(x[k] * inv)),  in [-127, 127]
+//
+// The definition is in these fp32 operations, so that host, device and any other program agree on
+// every code.  A row with an infinity or a NaN gets codes 0 and scale NaN: its products are NaN.
+#pragma once
+
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace smb {
+namespace qi8 {
+
+constexpr float kMinAmax = 7.8886090522101181e-31f;   // 2^-100
+
+// Eight consecutive elements as they are loaded.
+template <bool kBf16>
+struct Vec {
+  uint32_t w[kBf16 ? 4 : 8];
+};
+
+template <bool kBf16>
+__device__ __forceinline__ Vec<kBf16> load_vec(const void* row, int64_t k) {
+  Vec<kBf16> v;
+  const uint4* p = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + k * (kBf16 ? 2 : 4));
+#pragma unroll
+  for (int i = 0; i < (kBf16 ? 1 : 2); ++i) {
+    const uint4 q = p[i];
+    v.w[4 * i] = q.x;
+    v.w[4 * i + 1] = q.y;
+    v.w[4 * i + 2] = q.z;
+    v.w[4 * i + 3] = q.w;
+  }
+  return v;
+}
+
+// Largest magnitude as an fp32 bit pattern: magnitudes order like their bits, and infinities and
+// NaNs come out above every finite value.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t abs_max_bits(const Vec<kBf16>& v, uint32_t m) {
+  if (kBf16) {
+    uint32_t pair = v.w[0] & 0x7FFF7FFFu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) pair = __vmaxu2(pair, v.w[i] & 0x7FFF7FFFu);
+    return max(m, max(pair << 16, pair & 0xFFFF0000u));
+  }
+#pragma unroll
+  for (int i = 0; i < (kBf16 ? 4 : 8); ++i) m = max(m, v.w[i] & 0x7FFFFFFFu);
+  return m;
+}
+
+// Bits of the rounded code in the low byte: adding 1.5 * 2^23 to |q| <= 127 leaves no room for a
+// fraction, so the addition itself rounds half to even.
+__device__ __forceinline__ uint32_t code_bits(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
+
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint2 encode(const Vec<kBf16>& v, float inv) {
+  uint32_t c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float x;
+    if (kBf16) x = __uint_as_float((i & 1) ? (v.w[i >> 1] & 0xFFFF0000u) : (v.w[i >> 1] << 16));
+    else x = __uint_as_float(v.w[kBf16 ? 0 : i]);
+    c[i] = code_bits(x, inv);
+  }
+  return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float load_one(const void* row, int64_t k) {
+  if (kBf16) return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[k]) << 16);
+  return static_cast<const float*>(row)[k];
+}
+
+struct RowScale {
+  float scale, inv;
+  bool bad;
+};
+
+__host__ __device__ inline RowScale row_scale(float amax, bool finite) {
+  RowScale r;
+  r.bad = !finite;
+  const float a = amax > kMinAmax ? amax : kMinAmax;
+#ifdef __CUDA_ARCH__
+  r.scale = __fdiv_rn(a, 127.0f);
+  r.inv = __fdiv_rn(127.0f, a);
+#else
+  r.scale = a / 127.0f;
+  r.inv = 127.0f / a;
+#endif
+  return r;
+}
+
+// One row by `kThreads` threads of a CTA (32: a warp, no barrier; more: `red` holds one word per warp
+// of the CTA, and the CTA's threads belong to one row).  `store8(k, codes)` and `store1(k, code)`
+// receive the codes; returns the row's scale.  kVecs vectors per thread stay in registers between the
+// two passes, longer rows are read again (from L2).
+template <bool kBf16, int kThreads, int kVecs, bool kAligned, class Store8, class Store1>
+__device__ __forceinline__ float quantize_row(const void* row, int K, int tid, uint32_t* red, Store8 store8,
+                                              Store1 store1) {
+  const int nvec = kAligned ? K / 8 : 0;
+  Vec<kBf16> held[kVecs];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = tid + i * kThreads;
+    if (v < nvec) held[i] = load_vec<kBf16>(row, static_cast<int64_t>(v) * 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i)
+    if (tid + i * kThreads < nvec) m = abs_max_bits<kBf16>(held[i], m);
+  for (int v = tid + kVecs * kThreads; v < nvec; v += kThreads)
+    m = abs_max_bits<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), m);
+  for (int k = nvec * 8 + tid; k < K; k += kThreads)
+    m = max(m, __float_as_uint(load_one<kBf16>(row, k)) & 0x7FFFFFFFu);
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (kThreads > 32) {
+    if ((tid & 31) == 0) red[tid >> 5] = m;
+    __syncthreads();
+    m = red[tid & (kThreads / 32 - 1)];
+    m = __reduce_max_sync(0xffffffffu, m);
+  }
+  const RowScale rs = row_scale(__uint_as_float(m), m < 0x7F800000u);
+  const float inv = rs.inv;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const int v = tid + i * kThreads;
+    if (v < nvec) store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(held[i], inv));
+  }
+  for (int v = tid + kVecs * kThreads; v < nvec; v += kThreads)
+    store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), inv));
+  for (int k = nvec * 8 + tid; k < K; k += kThreads)
+    store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(load_one<kBf16>(row, k), inv) & 0xFFu));
+  return rs.bad ? __uint_as_float(0x7FC00000u) : rs.scale;
+}
+
+}  // namespace qi8
+}  // namespace smb

@@ -393,6 +393,127 @@ class Fp4HostContext:
             pass
 
 
+# ------------------------------------------------------------------------------- int8
+def quantize_i8_host(src: np.ndarray):
+    """FP32 [rows, K] -> (int8 codes [rows, K], fp32 scales [rows]), one scale per row."""
+    src = np.ascontiguousarray(src, dtype=np.float32)
+    rows, k = src.shape
+    codes = np.empty((rows, k), dtype=np.int8)
+    scales = np.empty(rows, dtype=np.float32)
+    capi.check(capi.lib().smb_quantize_i8_host(src.ctypes.data, k, codes.ctypes.data, k, scales.ctypes.data, rows, k))
+    return codes, scales
+
+
+def quantize_i8_device(src, codes, scales, rows: int, k: int, ld_src: int | None = None, ld_bytes: int | None = None,
+                       stream=None) -> None:
+    """FP32 rows on the device -> int8 codes and one scale per row."""
+    capi.check(capi.lib().smb_quantize_i8_device(
+        _ptr(src), k if ld_src is None else ld_src, _ptr(codes), k if ld_bytes is None else ld_bytes, _ptr(scales),
+        rows, k, _stream_ptr(stream)))
+
+
+def quantize_i8_bf16_device(src, codes, scales, rows: int, k: int, ld_src: int | None = None,
+                            ld_bytes: int | None = None, stream=None) -> None:
+    """BF16 rows on the device -> int8 codes and one scale per row."""
+    capi.check(capi.lib().smb_quantize_i8_bf16_device(
+        _ptr(src), k if ld_src is None else ld_src, _ptr(codes), k if ld_bytes is None else ld_bytes, _ptr(scales),
+        rows, k, _stream_ptr(stream)))
+
+
+def dense_gemm_i8_host(a: np.ndarray, sa: np.ndarray, b: np.ndarray, sb: np.ndarray) -> np.ndarray:
+    """Host arrays: A [M,K] int8, sa [M] f32, B [N,K] int8, sb [N] f32 -> D [M,N] bf16 bit patterns."""
+    a = np.ascontiguousarray(a, dtype=np.int8)
+    b = np.ascontiguousarray(b, dtype=np.int8)
+    sa = np.ascontiguousarray(sa, dtype=np.float32)
+    sb = np.ascontiguousarray(sb, dtype=np.float32)
+    if a.ndim != 2 or b.ndim != 2 or a.shape[1] != b.shape[1] or sa.shape != (a.shape[0],) or sb.shape != (b.shape[0],):
+        raise ValueError("A must be [M,K], B [N,K], and the scales [M] and [N]")
+    m, k = a.shape
+    n = b.shape[0]
+    d = np.empty((m, n), dtype=np.uint16)
+    capi.check(capi.lib().smb_dense_gemm_i8_host(a.ctypes.data, sa.ctypes.data, b.ctypes.data, sb.ctypes.data,
+                                                 d.ctypes.data, m, n, k))
+    return d
+
+
+class I8Plan:
+    """Tensor maps + tile choice for one (A, sa, B, sb, D) device buffer set: int8 operands, one scale
+    per row of A (token) and of B (channel), bf16 output."""
+
+    def __init__(self, a, sa, b, sb, d, m: int, n: int, k: int, lda: int | None = None, ldb: int | None = None,
+                 ldd: int | None = None, flags: int = 0):
+        self._lib = capi.lib()
+        self._h = C.c_void_p()
+        self.shape = (m, n, k)
+        self._keep = (a, sa, b, sb, d)
+        capi.check(self._lib.smb_i8_plan_create(
+            C.byref(self._h), _ptr(a), _ptr(sa), _ptr(b), _ptr(sb), _ptr(d), m, n, k, k if lda is None else lda,
+            k if ldb is None else ldb, self._out_pitch(n, flags) if ldd is None else ldd, flags))
+
+    @staticmethod
+    def _out_pitch(n: int, flags: int) -> int:
+        return n // 2 if flags & capi.FLAG_EPILOGUE_SWIGLU else n
+
+    @classmethod
+    def from_bf16_activations(cls, x, b, sb, d, m: int, n: int, k: int, ldx: int | None = None, ldb: int | None = None,
+                              ldd: int | None = None, flags: int = 0):
+        """Plan whose every run first quantises the BF16 activations `x` [M, K] on the device."""
+        self = cls.__new__(cls)
+        self._lib = capi.lib()
+        self._h = C.c_void_p()
+        self.shape = (m, n, k)
+        self._keep = (x, b, sb, d)
+        capi.check(self._lib.smb_i8_plan_create_bf16_activations(
+            C.byref(self._h), _ptr(x), k if ldx is None else ldx, _ptr(b), _ptr(sb), _ptr(d), m, n, k,
+            k if ldb is None else ldb, cls._out_pitch(n, flags) if ldd is None else ldd, flags))
+        return self
+
+    @classmethod
+    def grouped(cls, a, sa, b_stacked, sb_stacked, d, max_rows: int, n: int, k: int, groups: int, offsets,
+                lda: int | None = None, ldb: int | None = None, ldd: int | None = None, flags: int = 0):
+        """Grouped (mixture-of-experts) form; `offsets` is a device int32 array of groups + 1 row offsets that
+        every run reads (moe.dispatch_device writes it)."""
+        self = cls.__new__(cls)
+        self._lib = capi.lib()
+        self._h = C.c_void_p()
+        self.shape = (max_rows, n, k)
+        self._keep = (a, sa, b_stacked, sb_stacked, d, offsets)
+        capi.check(self._lib.smb_i8_grouped_plan_create(
+            C.byref(self._h), _ptr(a), _ptr(sa), _ptr(b_stacked), _ptr(sb_stacked), _ptr(d), max_rows, n, k,
+            k if lda is None else lda, k if ldb is None else ldb, cls._out_pitch(n, flags) if ldd is None else ldd,
+            groups, _ptr(offsets), flags))
+        return self
+
+    def tune(self, group_m: int = 0, max_clusters: int = 0) -> None:
+        capi.check(self._lib.smb_i8_plan_tune(self._h, group_m, max_clusters))
+
+    def run(self, stream=None) -> None:
+        capi.check(self._lib.smb_i8_plan_run(self._h, _stream_ptr(stream)))
+
+    def describe(self) -> str:
+        buf = C.create_string_buffer(160)
+        capi.check(self._lib.smb_i8_plan_describe(self._h, buf, 160))
+        return buf.value.decode()
+
+    def wait_probe(self, budget_cycles: int = 200_000, stream=None) -> None:
+        """Self test of the bounded device waits: the next check() raises SMB_ERR_DEVICE."""
+        capi.check(self._lib.smb_i8_plan_wait_probe(self._h, budget_cycles, _stream_ptr(stream)))
+
+    def check(self, stream=None) -> None:
+        capi.check(self._lib.smb_i8_plan_check(self._h, _stream_ptr(stream)))
+
+    def close(self) -> None:
+        if self._h:
+            self._lib.smb_i8_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Comm:
     """One rank's NCCL communicator behind the C ABI (one process per GPU)."""
 

@@ -1,0 +1,177 @@
+"""int8 product, routing and row sorting without a GPU: host quantiser, descriptor bits, refusals."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+
+def test_host_quantizer_matches_numpy(smb):
+    rng = np.random.default_rng(3)
+    x = (rng.standard_normal((60, 333)) * np.exp(rng.standard_normal((60, 1)))).astype(np.float32)
+    x[0] = 0.0
+    x[1] = np.float32(1e-38)                  # below the floor of amax: codes 0
+    x[2, :5] = [127, -127, 0.5, 1.5, 2.5]     # ties go to the even code
+    x[2, 5:] = 0
+    x[3, 7] = np.inf
+    x[4, 8] = -np.nan
+    x[5] *= np.float32(1e30)
+    codes, scales = smb.gemm.quantize_i8_host(x)
+    amax = np.maximum(np.abs(x).max(1), np.float32(2.0 ** -100)).astype(np.float32)
+    bad = ~np.isfinite(x).all(1)
+    with np.errstate(all="ignore"):
+        want = np.rint(x * (np.float32(127) / amax)[:, None])
+    want[bad] = 0
+    np.testing.assert_array_equal(codes, want.astype(np.int8))
+    np.testing.assert_array_equal(scales[~bad], (amax / np.float32(127))[~bad])
+    assert np.isnan(scales[bad]).all()
+    np.testing.assert_array_equal(codes[2, :5], [127, -127, 0, 2, 2])
+    ok = ~bad
+    # Half a code, and the rounding of x * inv at the top of the range (127 steps of 2^-24).
+    err = np.abs(codes[ok].astype(np.float64) * scales[ok, None].astype(np.float64) - x[ok])
+    assert (err <= scales[ok, None].astype(np.float64) * (0.5 + 3 * 127 * 2.0 ** -24)).all()
+
+
+def test_max_rows(smb):
+    f = smb.moe.max_rows
+    assert f(16, 8, 256) == 128 and f(0, 8, 4, 256) == 0
+    assert f(1, 1, 8, 256) == 256 and f(3, 2, 4, 256) == 4 * 256
+    assert f(100, 2, 4, 128) == (200 + 4 * 127) // 128 * 128
+    rng = np.random.default_rng(0)
+    for _ in range(200):
+        t, k, g, a = int(rng.integers(1, 60)), int(rng.integers(1, 9)), int(rng.integers(1, 20)), int(rng.choice([1, 4, 128, 256]))
+        counts = rng.multinomial(t * k, rng.dirichlet(np.full(g, 0.3)))
+        assert sum(-(-c // a) * a for c in counts) <= f(t, k, g, a)
+
+
+P = C.c_void_p(0x10000)        # stands for a device address; nothing here gets as far as using it
+ODD = C.c_void_p(0x10001)
+
+
+def _refused(smb, rc, text, code=None):
+    assert rc in ((code,) if code is not None else (smb.capi.SMB_ERR_INVALID, smb.capi.SMB_ERR_UNSUPPORTED)), rc
+    assert text in smb.capi.last_error(), smb.capi.last_error()
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(a=None), "null operand"), (dict(sa=None), "null operand"), (dict(b=None), "null operand"),
+    (dict(sb=None), "null operand"), (dict(d=None), "null operand"), (dict(M=0), "positive"), (dict(N=-1), "positive"),
+    (dict(K=0), "positive"), (dict(K=131072, lda=131072, ldb=131072), "int32"), (dict(lda=120), "lda"), (dict(lda=136), "lda"),
+    (dict(ldb=127), "ldb"), (dict(ldd=255), "ldd"), (dict(d=ODD), "2-byte"), (dict(sa=C.c_void_p(0x10002)), "4-byte"),
+    (dict(sb=C.c_void_p(0x10002)), "4-byte"), (dict(flags=256), "no int8 form"), (dict(flags=32), "no int8 form"),
+    (dict(flags=8192, N=255), "even N"),
+])
+def test_i8_plan_refusals(smb, change, text):
+    args = dict(a=P, sa=P, b=P, sb=P, d=P, M=64, N=256, K=128, lda=128, ldb=128, ldd=256, flags=0)
+    args.update(change)
+    h = C.c_void_p()
+    rc = smb.capi.lib().smb_i8_plan_create(C.byref(h), *args.values())
+    _refused(smb, rc, text)
+    assert not h.value
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(off=None), "null offsets"), (dict(off=C.c_void_p(0x10002)), "4-byte"), (dict(groups=0), "groups"),
+    (dict(groups=513), "groups"), (dict(rows=0), "positive"), (dict(rows=(8 << 20) + 1), "max_rows"),
+    (dict(groups=512, N=1 << 23, ldd=1 << 23), "too large"),
+])
+def test_i8_grouped_plan_refusals(smb, change, text):
+    args = dict(a=P, sa=P, b=P, sb=P, d=P, rows=64, N=256, K=128, lda=128, ldb=128, ldd=256, groups=4, off=P, flags=0)
+    args.update(change)
+    if args["ldd"] < args["N"]:
+        args["ldd"] = args["N"]
+    h = C.c_void_p()
+    rc = smb.capi.lib().smb_i8_grouped_plan_create(C.byref(h), *args.values())
+    _refused(smb, rc, text)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(x=None), "null activations"), (dict(ldx=100), "pitch"), (dict(x=ODD), "2-byte"), (dict(K=131072, ldb=131072), "int32"),
+])
+def test_i8_activation_plan_refusals(smb, change, text):
+    args = dict(x=P, ldx=131072, b=P, sb=P, d=P, M=64, N=256, K=128, ldb=128, ldd=256, flags=0)
+    args.update(change)
+    h = C.c_void_p()
+    rc = smb.capi.lib().smb_i8_plan_create_bf16_activations(C.byref(h), *args.values())
+    _refused(smb, rc, text)
+
+
+def test_i8_null_handles_and_host_refusals(smb):
+    lib = smb.capi.lib()
+    inv = smb.capi.SMB_ERR_INVALID
+    assert lib.smb_i8_plan_run(None, None) == inv and lib.smb_i8_plan_check(None, None) == inv
+    assert lib.smb_i8_plan_tune(None, 0, 0) == inv and lib.smb_i8_plan_destroy(None) == 0
+    assert lib.smb_i8_plan_create(None, P, P, P, P, P, 1, 1, 16, 16, 16, 8, 0) == inv
+    assert lib.smb_dense_gemm_i8_host(None, P, P, P, P, 1, 1, 1) == inv
+    with pytest.raises(ValueError):
+        smb.gemm.dense_gemm_i8_host(np.zeros((2, 3), np.int8), np.zeros(2, np.float32), np.zeros((2, 4), np.int8),
+                                    np.zeros(2, np.float32))
+    x = np.zeros((2, 8), np.float32)
+    c, s = np.zeros((2, 8), np.int8), np.zeros(2, np.float32)
+    q = lib.smb_quantize_i8_host
+    assert q(None, 8, c.ctypes.data, 8, s.ctypes.data, 2, 8) == inv
+    assert q(x.ctypes.data, 7, c.ctypes.data, 8, s.ctypes.data, 2, 8) == inv
+    assert q(x.ctypes.data, 8, c.ctypes.data, 7, s.ctypes.data, 2, 8) == inv
+    assert q(x.ctypes.data, 8, c.ctypes.data, 8, s.ctypes.data, 2, 0) == inv
+    assert q(x.ctypes.data, 8, c.ctypes.data, 8, s.ctypes.data, 0, 8) == 0
+    assert lib.smb_quantize_i8_bf16_device(ODD, 8, P, 8, P, 2, 8, None) == inv
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(logits=None), "null logits"), (dict(dtype=2), "dtype"), (dict(logits=C.c_void_p(0x10002)), "aligned"),
+    (dict(tokens=-1), "negative"), (dict(experts=513), "experts"), (dict(experts=0), "experts"), (dict(top_k=0), "top_k"),
+    (dict(top_k=33), "top_k"), (dict(experts=4, n_groups=1, top_groups=1, top_k=5), "top_k"), (dict(ld=63), "pitch"),
+    (dict(n_groups=3), "groups"), (dict(n_groups=64), "groups"), (dict(n_groups=0), "groups"), (dict(top_groups=0), "top_groups"),
+    (dict(top_groups=9), "top_groups"), (dict(top_groups=1, top_k=9), "open groups"), (dict(flags=8), "flags"),
+    (dict(ids=None), "null output"), (dict(weights=None), "null output"),
+])
+def test_route_refusals(smb, change, text):
+    args = dict(logits=P, dtype=0, ld=64, bias=None, tokens=8, experts=64, top_k=4, n_groups=8, top_groups=4, flags=0, scale=1.0,
+                ids=P, weights=P, stream=None)
+    args.update(change)
+    _refused(smb, smb.capi.lib().smb_moe_route_device(*args.values()), text)
+
+
+def test_empty_calls_are_valid(smb):
+    lib = smb.capi.lib()
+    assert lib.smb_moe_route_device(P, 0, 64, None, 0, 64, 4, 1, 1, 0, 1.0, P, P, None) == 0
+    assert lib.smb_moe_route_backward_device(P, 0, 64, P, P, 0, 64, 4, 0, 1.0, P, 64, None) == 0
+    assert lib.smb_moe_gather_bf16_device(P, 8, P, 0, 1, 8, 4, P, 8, None) == 0
+    assert lib.smb_moe_gather_i8_device(P, 8, P, 0, 1, 8, 4, P, 8, P, None) == 0
+    assert lib.smb_moe_combine_device(P, 8, P, P, 0, 1, 8, 4, P, 8, None) == 0
+    # The address of an empty tensor is null.
+    assert lib.smb_moe_route_device(None, 0, 64, None, 0, 64, 4, 1, 1, 0, 1.0, None, None, None) == 0
+    assert lib.smb_moe_gather_bf16_device(None, 8, None, 0, 1, 8, 0, None, 8, None) == 0
+    assert lib.smb_quantize_i8_bf16_device(None, 8, None, 8, None, 0, 8, None) == 0
+    assert lib.smb_moe_combine_backward_device(P, 8, P, 8, P, P, 0, 1, 8, 4, P, 8, P, None) == 0
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(ids=None), "null"), (dict(offsets=None), "null"), (dict(row_of_slot=None), "null"), (dict(slot_of_row=None), "null"),
+    (dict(ids=C.c_void_p(0x10002)), "4-byte"), (dict(groups=0), "groups"), (dict(groups=1025), "groups"), (dict(tokens=-1), "extents"),
+    (dict(top_k=0), "extents"), (dict(top_k=33), "extents"), (dict(align=0), "alignment"), (dict(max_rows=63), "room"),
+    (dict(align=256, max_rows=1023), "room"), (dict(tiles=P), "256"), (dict(tokens=1 << 29, max_rows=1 << 31), "slots"),
+])
+def test_dispatch_refusals(smb, change, text):
+    args = dict(ids=P, tokens=16, top_k=4, groups=4, align=1, max_rows=64, offsets=P, row_of_slot=P, slot_of_row=P, tiles=None,
+                stream=None)
+    args.update(change)
+    _refused(smb, smb.capi.lib().smb_moe_dispatch_device(*args.values()), text)
+
+
+def test_row_copy_refusals(smb):
+    lib = smb.capi.lib()
+    base = dict(x=P, ld_x=64, row=P, tokens=4, top_k=2, width=64, max_rows=8, out=P, ld_out=64, stream=None)
+    for change, text in [(dict(x=None), "null"), (dict(out=None), "null"), (dict(row=None), "null"), (dict(ld_x=63), "pitch"),
+                         (dict(ld_out=63), "pitch"), (dict(width=0), "width"), (dict(top_k=33), "top_k"), (dict(max_rows=0), "capacity"),
+                         (dict(x=ODD), "2-byte"), (dict(tokens=-1), "token count"), (dict(row=ODD), "4-byte")]:
+        args = dict(base, **change)
+        _refused(smb, lib.smb_moe_gather_bf16_device(*args.values()), text)
+        _refused(smb, lib.smb_moe_combine_device(args["x"], args["ld_x"], args["row"], P, args["tokens"], args["top_k"],
+                                                 args["width"], args["max_rows"], args["out"], args["ld_out"], None), text)
+    _refused(smb, lib.smb_moe_gather_i8_device(P, 64, P, 4, 2, 64, 8, P, 63, P, None), "pitch")
+    _refused(smb, lib.smb_moe_gather_i8_device(P, 64, P, 4, 2, 64, 8, P, 64, None, None), "null")
+    _refused(smb, lib.smb_moe_combine_backward_device(P, 64, None, 64, P, P, 4, 2, 64, 8, P, 64, P, None), "needs the rows")
+    _refused(smb, lib.smb_moe_combine_backward_device(P, 64, P, 64, P, P, 4, 2, 64, 8, None, 64, P, None), "null")
+    _refused(smb, lib.smb_moe_combine_backward_device(P, 64, P, 64, P, P, 4, 2, 64, 8, P, 60, P, None), "pitch")
+    _refused(smb, lib.smb_moe_route_backward_device(P, 0, 64, None, P, 4, 64, 2, 0, 1.0, P, 64, None), "null")
+    _refused(smb, lib.smb_moe_route_backward_device(P, 0, 64, P, P, 4, 64, 2, 0, 1.0, P, 63, None), "pitch")
