@@ -449,7 +449,7 @@ int smb_quantize_i8_host(const float* src, int64_t ld_src, int8_t* codes, int64_
                          int64_t rows, int64_t K);
 
 /* Plans as for the BF16 GEMM.  Flags: SMB_FLAG_FORCE_PLAIN_STORE, _TILE_N_128 / _256 / _512,
- * _NO_DECODE, _EPILOGUE_SWIGLU (rows of B interleaved, even = up, odd = gate, D [M, N / 2] =
+ * _NO_DECODE, _DECODE_SINGLE (force the kernel for few rows), _EPILOGUE_SWIGLU (rows of B interleaved, even = up, odd = gate, D [M, N / 2] =
  * bf16(silu(gate) * up) of the scaled sums, silu accurate to fp32), _WEIGHTS_STATIC; others are
  * refused. */
 typedef struct smb_i8_plan smb_i8_plan;

@@ -21,7 +21,7 @@ namespace {
 
 constexpr unsigned kKnownFlags = SMB_FLAG_FORCE_PLAIN_STORE | SMB_FLAG_TILE_N_128 | SMB_FLAG_TILE_N_256 |
                                  SMB_FLAG_TILE_N_512 | SMB_FLAG_NO_DECODE | SMB_FLAG_EPILOGUE_SWIGLU |
-                                 SMB_FLAG_WEIGHTS_STATIC;
+                                 SMB_FLAG_WEIGHTS_STATIC | SMB_FLAG_DECODE_SINGLE;
 
 struct I8Args {
   const void* a;
@@ -107,6 +107,9 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
       rc = set_error(SMB_ERR_UNSUPPORTED, "i8 plan: the gated epilogue needs a 16-byte-aligned D with ldd %% 8 == 0");
     L.tile_n = 256;
   }
+  const bool tiled_only = (g.flags & (SMB_FLAG_NO_DECODE | SMB_FLAG_TILE_N_128 | SMB_FLAG_TILE_N_256 | SMB_FLAG_TILE_N_512)) != 0;
+  L.decode = !tiled_only && i8_pick_decode(g.M, g.N, g.K, g.offsets != nullptr ? (g.groups < 2 ? 2 : g.groups) : 1,
+                                           (g.flags & SMB_FLAG_DECODE_SINGLE) != 0, &L.chunk, &L.box_rows);
   const void* a = g.a;
   int64_t lda = g.lda;
   L.sa = g.sa;
@@ -123,10 +126,11 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
     }
     if (e != cudaSuccess) rc = set_cuda_error(e, "i8 plan: allocation");
   }
-  if (rc == SMB_OK) rc = encode_tmap_2d(&L.tmap_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, 128, 128, true);
+  if (rc == SMB_OK) rc = encode_tmap_2d(&L.tmap_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, L.decode ? L.box_rows : 128, 128,
+                        true);
   if (rc == SMB_OK)
     rc = encode_tmap_2d(&L.tmap_b, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, static_cast<uint64_t>(g.groups) * g.N, g.K, g.ldb,
-                        L.tile_n / 2, 128, true);
+                        L.decode ? 128 : L.tile_n / 2, 128, true);
   if (rc == SMB_OK) {
     if (L.tma_store)
       rc = encode_tmap_2d(&L.tmap_d, g.d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, g.M, L.swiglu ? g.N / 2 : g.N, g.ldd * 2, 32,
@@ -193,7 +197,7 @@ extern "C" int smb_i8_plan_run(smb_i8_plan* plan, void* stream) {
                                 L.K, st);
     if (rc != SMB_OK) return rc;
   }
-  return i8_launch(plan->launch, st);
+  return plan->launch.decode ? i8_decode_launch(plan->launch, st) : i8_launch(plan->launch, st);
 }
 
 extern "C" int smb_i8_plan_check(smb_i8_plan* plan, void* stream) {
@@ -213,6 +217,11 @@ extern "C" int smb_i8_plan_check(smb_i8_plan* plan, void* stream) {
 extern "C" int smb_i8_plan_describe(smb_i8_plan* plan, char* out, size_t capacity) {
   if (plan == nullptr || out == nullptr || capacity == 0) return set_error(SMB_ERR_INVALID, "i8 plan describe: null argument");
   const I8Launch& L = plan->launch;
+  if (L.decode) {
+    snprintf(out, capacity, "i8 decode chunk=%d%s%s%s", L.chunk, L.swiglu ? " swiglu" : "",
+             L.offsets != nullptr ? " grouped" : "", plan->act_src != nullptr ? " bf16-activations" : "");
+    return SMB_OK;
+  }
   snprintf(out, capacity, "i8 tile 256x%d store=%s%s%s", L.tile_n * L.sub_blocks,
            L.swiglu ? "swiglu" : (L.tma_store ? "tma" : "plain"), L.offsets != nullptr ? " grouped" : "",
            plan->act_src != nullptr ? " bf16-activations" : "");

@@ -1,0 +1,492 @@
+// int8 GEMM for few rows per weight matrix (decode batches, experts with a handful of tokens): bound by
+// reading B once.  Same result, bit for bit, as gemm_i8.cu.
+//
+// The operands swap roles: 128 rows of B (output channels) fill the rows of a 1-CTA tcgen05.mma and up
+// to 128 rows of A (tokens) its columns, so the instruction does no more work than the tokens need and a
+// stage is mostly weights.  Accumulator lane = channel, column = token.
+//
+// One CTA per SM walks the (row chunk, channel tile) pairs; warp 0 loads (TMA), warp 1 issues the MMAs,
+// warps 2-5 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs cuts the K loop of a
+// pair and adds its int32 partial sums through distributed shared memory: the sums are exact, so their
+// order does not matter, and there is neither workspace nor atomic.
+#include "gemm_common.cuh"
+#include "i8_common.cuh"
+#include "i8_epilogue.cuh"
+#include "ptx.cuh"
+
+namespace smb {
+
+namespace i8d {
+
+constexpr int kTileRows = 128;        // channels per tile
+constexpr int kBlockK = 128;
+constexpr int kThreads = 192;
+constexpr int kWBytes = kTileRows * kBlockK;
+constexpr int kMaxStages = 12;
+constexpr int kBarBytes = 256;
+constexpr int kTableBytes = (kI8MaxGroups + 8) * 4;
+// The whole of shared memory, whatever the ring needs: no other kernel that allocates tensor memory can
+// then share the SM, so no allocation ever waits for a CTA that waits for this kernel to end.
+constexpr int kTotal = 232448;
+constexpr int kRingBudget = kTotal - 1024 - kBarBytes - kTableBytes;
+
+struct Params {
+  int M, N, K;
+  int tiles_n;
+  int chunk;          // tokens per tile, a multiple of 16 up to 128
+  int box_rows;       // tokens per TMA box: the chunk, or 16 where groups are ragged
+  int stages, stage_bytes;
+  int tmem_cols, bank_cols;
+  int kb_per;         // K blocks per CTA of a cluster
+  int ldd;
+  uint16_t* d_ptr;
+  const float* sa;
+  const float* sb;
+  const int* offsets;
+  int groups;
+  int* status;
+  int weights_static;
+};
+
+struct Tile {
+  int row0, rows;     // tokens [row0, row0 + rows)
+  int group, col0;    // channels [col0, col0 + 128) of the group
+};
+
+__device__ __forceinline__ void group_rows(const Params& p, int g, int& lo, int& hi) {
+  if (p.offsets == nullptr) {
+    lo = 0;
+    hi = p.M;
+    return;
+  }
+  lo = min(max(ld_global_s32(p.offsets + g), 0), p.M);
+  hi = min(max(ld_global_s32(p.offsets + g + 1), lo), p.M);
+}
+
+// Number of row chunks before every group, groups + 1 words at `table`.  First warp of the CTA.
+__device__ __forceinline__ void build_chunks(const Params& p, int* table, int lane) {
+  constexpr int kPer = kI8MaxGroups / 32;
+  int count[kPer];
+  int sum = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int g = lane * kPer + i;
+    int lo = 0, hi = 0;
+    if (g < p.groups) group_rows(p, g, lo, hi);
+    count[i] = (hi - lo + p.chunk - 1) / p.chunk;
+    sum += count[i];
+  }
+  int before = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, before, d);
+    if (lane >= d) before += up;
+  }
+  before -= sum;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int g = lane * kPer + i;
+    if (g <= p.groups) table[g] = before;
+    before += count[i];
+  }
+  if (lane == 31 && p.groups == kI8MaxGroups) table[kI8MaxGroups] = before;
+}
+
+// Tiles of a group run chunk-fastest: the chunks that read the same weights are neighbours in time.
+__device__ __forceinline__ Tile find_tile(const Params& p, const int* table, int t, int lane) {
+  constexpr int kPer = kI8MaxGroups / 32;
+  const int c = t / p.tiles_n;
+  int g = 0;
+  if (p.groups > 1) {
+    const int first = lane * kPer;
+    const unsigned seg_mask = __ballot_sync(0xffffffffu, first < p.groups && table[min(first, p.groups)] <= c);
+    const int seg = 31 - __clz(seg_mask | 1u);
+    const int g0 = seg * kPer + (lane & (kPer - 1));
+    const unsigned in_mask = __ballot_sync(0xffffffffu, lane < kPer && g0 < p.groups && table[min(g0, p.groups)] <= c);
+    g = seg * kPer + 31 - __clz(in_mask | 1u);
+  }
+  const int chunks = table[g + 1] - table[g];
+  const int local = t - table[g] * p.tiles_n;
+  const int nt = local / chunks;
+  int lo, hi;
+  group_rows(p, g, lo, hi);
+  Tile r;
+  r.group = g;
+  r.col0 = nt * kTileRows;
+  r.row0 = lo + (local - nt * chunks) * p.chunk;
+  r.rows = min(p.chunk, hi - r.row0);
+  return r;
+}
+
+// Two tokens (rows m, m + 1 of D) of this lane's channel n, already scaled.  Neighbouring lanes trade
+// halves, so that even lanes write two channels of row m and odd lanes two of row m + 1; with the gated
+// epilogue the two are up and gate of one output.
+template <bool kSwiglu, bool kPairs>
+__device__ __forceinline__ void store_pair(const Params& p, long long m, int valid, int n, float z0, float z1) {
+  if (!kSwiglu && !kPairs) {
+    if (n < p.N) {
+      if (valid > 0) p.d_ptr[m * p.ldd + n] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(z0), 0u) & 0xFFFFu);
+      if (valid > 1) p.d_ptr[(m + 1) * p.ldd + n] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(z1), 0u) & 0xFFFFu);
+    }
+    return;
+  }
+  const bool odd = n & 1;
+  const float other = __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
+  const float lo = odd ? other : z0, hi = odd ? z1 : other;
+  const int n0 = n & ~1;
+  if (valid <= (odd ? 1 : 0) || n0 >= p.N) return;
+  uint16_t* row = p.d_ptr + (m + (odd ? 1 : 0)) * p.ldd;
+  if (kSwiglu) {
+    row[n0 >> 1] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(silu_mul(hi, lo)), 0u) & 0xFFFFu);
+  } else {
+    const uint32_t v = pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi));
+    if (n0 + 1 < p.N) *reinterpret_cast<uint32_t*>(row + n0) = v;
+    else row[n0] = static_cast<uint16_t>(v & 0xFFFFu);
+  }
+}
+
+// kSplit: the CTAs of a cluster share the K loop of ONE tile (the grid has a cluster for every tile).
+template <bool kSwiglu, bool kPairs, bool kSplit>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                      const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t ring_base = smem_base;
+  const uint32_t bar_base = ring_base + kRingBudget / 1024 * 1024;
+  int* table = reinterpret_cast<int*>(smem_raw + (bar_base + kBarBytes - smem_u32(smem_raw)));
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (kMaxStages + s); };
+  auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStages + b); };
+  auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStages + 2 + b); };
+  const uint32_t tmem_slot = bar_base + 8u * (2 * kMaxStages + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int split = kSplit ? static_cast<int>(cluster_nctarank()) : 1;
+  const int rank = kSplit ? static_cast<int>(cluster_ctarank()) : 0;
+  const int unit = blockIdx.x / split;
+  const int units = gridDim.x / split;
+  const int num_kb = (p.K + kBlockK - 1) / kBlockK;
+  const int kb0 = rank * p.kb_per;
+  const int kb1 = min(num_kb, kb0 + p.kb_per);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full_bar(b), 1);
+      mbar_init(acc_empty_bar(b), 4);
+    }
+    fence_mbar_init_cluster();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_w);
+    tma_prefetch_desc(&tmap_x);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(tmem_slot, p.tmem_cols);
+    tmem_relinquish<1>();
+  }
+  const bool grouped = p.offsets != nullptr;
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  griddep_launch_dependents();   // not before this CTA holds its tensor memory
+  const uint64_t pol_w = l2_policy_evict_first();
+  const uint64_t pol_x = l2_policy_evict_last();
+  // Weights that nobody on the stream writes are on their way while the kernel that makes the
+  // activations still runs: the first ring's worth of the first tile (a plain product knows its tiles).
+  int early = 0;
+  if (!grouped && p.weights_static) {
+    early = min(p.stages, kb1 - kb0);
+    if (warp == 0) {
+      const int nt = unit / ((p.M + p.chunk - 1) / p.chunk);
+      const int rows = min(p.chunk, p.M);   // every chunk is loaded as whole boxes
+      const uint32_t bytes = kWBytes + ((rows + p.box_rows - 1) / p.box_rows) * p.box_rows * kBlockK;
+      for (int s = 0; s < early; ++s) {
+        if (elect_one()) {
+          mbar_arrive_expect_tx(full_bar(s), bytes);
+          tma_load_2d_cta_hint(ring_base + s * p.stage_bytes, &tmap_w, full_bar(s), (kb0 + s) * kBlockK, nt * kTileRows, pol_w);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  griddep_wait();
+  if (grouped) {
+    if (warp == 0) build_chunks(p, table, lane);
+  } else if (threadIdx.x == 0) {
+    table[0] = 0;
+    table[1] = (p.M + p.chunk - 1) / p.chunk;
+  }
+  __syncthreads();
+  uint32_t tmem_base;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
+  int num_tiles = table[p.groups] * p.tiles_n;
+  if (kSplit) num_tiles = min(num_tiles, units);   // offsets that overlap could ask for more
+
+  if (warp == 0) {
+    // ------------------------------------------------------------- TMA producer
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    for (int t = unit; t < num_tiles && ok; t += units) {
+      const Tile tile = find_tile(p, table, t, lane);
+      const int boxes = (tile.rows + p.box_rows - 1) / p.box_rows;
+      const uint32_t bytes = kWBytes + boxes * p.box_rows * kBlockK;
+      const int row_w = tile.group * p.N + tile.col0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(empty_bar(s), ph ^ 1u)) {
+          report_status(p.status, kDevTimeoutProducer);
+          ok = false;
+          break;
+        }
+        const uint32_t dst = ring_base + s * p.stage_bytes;
+        if (elect_one()) {
+          if (early == 0) {
+            mbar_arrive_expect_tx(full_bar(s), bytes);
+            tma_load_2d_cta_hint(dst, &tmap_w, full_bar(s), kb * kBlockK, row_w, pol_w);
+          }
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d_cta_hint(dst + kWBytes + b * p.box_rows * kBlockK, &tmap_x, full_bar(s), kb * kBlockK,
+                                 tile.row0 + b * p.box_rows, pol_x);
+        }
+        if (early > 0) --early;
+        __syncwarp();
+        if (++s == p.stages) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (!ok) {
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies in flight land before shared memory goes away
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------- MMA issue
+    int s = 0;
+    uint32_t ph = 0;
+    int local = 0;
+    bool ok = true;
+    for (int t = unit; t < num_tiles && ok; t += units, ++local) {
+      const Tile tile = find_tile(p, table, t, lane);
+      const int boxes = (tile.rows + p.box_rows - 1) / p.box_rows;
+      const uint32_t idesc = make_idesc_i8(128, boxes * p.box_rows);
+      const int bank = local & 1;
+      if (!mbar_wait(acc_empty_bar(bank), (static_cast<uint32_t>(local >> 1) & 1u) ^ 1u)) {
+        report_status(p.status, kDevTimeoutMmaAcc);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(bank * p.bank_cols);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(full_bar(s), ph)) {
+          report_status(p.status, kDevTimeoutMmaFull);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t w_addr = ring_base + s * p.stage_bytes;
+        const uint64_t desc_w = make_smem_desc(w_addr, 1024, 16, kSwizzle128B);
+        const uint64_t desc_x = make_smem_desc(w_addr + kWBytes, 1024, 16, kSwizzle128B);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k)
+            mma_i8_ss<1>(tmem_d, desc_w + 2u * k, desc_x + 2u * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+          mma_commit_1cta(empty_bar(s));
+        }
+        __syncwarp();
+        if (++s == p.stages) { s = 0; ph ^= 1u; }
+      }
+      if (ok && elect_one()) mma_commit_1cta(acc_full_bar(bank));
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------- epilogue (4 warps)
+    const int quarter = warp & 3;
+    int local = 0;
+    for (int t = unit; t < num_tiles; t += units, ++local) {
+      const Tile tile = find_tile(p, table, t, lane);
+      const int bank = local & 1;
+      const int n = tile.col0 + quarter * 32 + lane;
+      const float sb = n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
+      if (!mbar_wait(acc_full_bar(bank), static_cast<uint32_t>(local >> 1) & 1u)) {
+        if (lane == 0) report_status(p.status, kDevTimeoutEpilogue);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(bank * p.bank_cols);
+      for (int c0 = 0; c0 < tile.rows; c0 += 16) {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(taddr + c0, v);
+        tmem_ld_wait();
+        if (kSplit) {
+          // The ring is idle: its only tile's MMAs are complete.  [token][channel] words.
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring_base + ((c0 + i) * kTileRows + quarter * 32 + lane) * 4), "r"(v[i])
+                         : "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const int c = c0 + i;
+            if (c < tile.rows) {
+              const float s0 = p.sa[tile.row0 + c];
+              const float s1 = c + 1 < tile.rows ? p.sa[tile.row0 + c + 1] : 0.0f;
+              store_pair<kSwiglu, kPairs>(p, tile.row0 + c, tile.rows - c, n, scale_i32(v[i], s0, sb), scale_i32(v[i + 1], s1, sb));
+            }
+          }
+        }
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty_bar(bank));
+    }
+  }
+  __syncwarp();
+  if (kSplit) {
+    cluster_sync_all();
+    if (warp >= 2 && unit < num_tiles) {
+      // CTA r of the cluster owns tokens [r * per, (r + 1) * per) of the tile.
+      const Tile tile = find_tile(p, table, unit, lane);
+      const int quarter = warp & 3;
+      const int n = tile.col0 + quarter * 32 + lane;
+      const float sb = n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
+      const int per = ((p.chunk + split - 1) / split + 1) & ~1;
+      const int end = min(tile.rows, (rank + 1) * per);
+      for (int c = rank * per; c < end; c += 2) {
+        uint32_t a0 = 0, a1 = 0;
+        const uint32_t addr = ring_base + (c * kTileRows + quarter * 32 + lane) * 4;
+        for (int q = 0; q < split; ++q) {
+          const uint32_t remote = mapa_u32(addr, q);
+          a0 += ld_shared_cluster_u32(remote);
+          a1 += ld_shared_cluster_u32(remote + kTileRows * 4);
+        }
+        const float s0 = p.sa[tile.row0 + c];
+        const float s1 = c + 1 < tile.rows ? p.sa[tile.row0 + c + 1] : 0.0f;
+        store_pair<kSwiglu, kPairs>(p, tile.row0 + c, end - c, n, scale_i32(a0, s0, sb), scale_i32(a1, s1, sb));
+      }
+    }
+    cluster_sync_all();   // partial sums stay until every CTA has read them
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc<1>(tmem_base, p.tmem_cols);
+  }
+}
+
+}  // namespace i8d
+
+namespace {
+
+template <bool kSwiglu, bool kPairs, bool kSplit>
+int launch_i8_decode(const I8Launch& L, const i8d::Params& p, int ctas, int split, cudaStream_t stream) {
+  auto kernel = i8d::gemm_i8_decode_kernel<kSwiglu, kPairs, kSplit>;
+  static thread_local int configured_device = -1;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return set_error(SMB_ERR_CUDA, "cudaGetDevice failed");
+  if (configured_device != dev) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, i8d::kTotal);
+    if (e != cudaSuccess) return set_cuda_error(e, "cudaFuncSetAttribute(i8 decode smem)");
+    configured_device = dev;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.blockDim = dim3(i8d::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = i8d::kTotal;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = kSplit ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L.tmap_b, L.tmap_a, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e, "i8 decode GEMM launch");
+  return SMB_OK;
+}
+
+}  // namespace
+
+bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows) {
+  (void)N;
+  (void)K;
+  if (groups == 1) {
+    if (M > 128 && !force) return false;
+    *chunk = M >= 128 ? 128 : (M + 15) / 16 * 16;
+    *box_rows = *chunk;
+    return true;
+  }
+  const int average = (M + groups - 1) / groups;
+  if (average > 32 && !force) return false;
+  *chunk = average <= 8 ? 16 : (average <= 16 ? 32 : 64);
+  if (average > 64) *chunk = 128;
+  *box_rows = 16;
+  return true;
+}
+
+int i8_decode_launch(const I8Launch& L, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return set_error(SMB_ERR_CUDA, "i8 decode: no current device");
+  if (L.max_clusters > 0 && sms > 2 * L.max_clusters) sms = 2 * L.max_clusters;
+  i8d::Params p = {};
+  p.M = L.M;
+  p.N = L.N;
+  p.K = L.K;
+  p.tiles_n = (L.N + i8d::kTileRows - 1) / i8d::kTileRows;
+  p.chunk = L.chunk;
+  p.box_rows = L.box_rows;
+  p.stage_bytes = i8d::kWBytes + L.chunk * i8d::kBlockK;
+  p.stages = i8d::kRingBudget / 1024 * 1024 / p.stage_bytes;
+  if (p.stages > i8d::kMaxStages) p.stages = i8d::kMaxStages;
+  p.bank_cols = L.chunk <= 16 ? 16 : (L.chunk <= 32 ? 32 : (L.chunk <= 64 ? 64 : 128));
+  p.tmem_cols = 2 * p.bank_cols;
+  p.ldd = L.ldd;
+  p.d_ptr = static_cast<uint16_t*>(L.d);
+  p.sa = L.sa;
+  p.sb = L.sb;
+  p.offsets = L.offsets;
+  p.groups = L.groups;
+  p.status = L.status;
+  p.weights_static = L.weights_static ? 1 : 0;
+  // Upper bound of the (chunk, channel tile) pairs; exact for a plain product.
+  const long long full = (static_cast<long long>(L.M) + L.chunk - 1) / L.chunk;
+  long long chunks = full;
+  if (L.offsets != nullptr) chunks = L.M / L.chunk + (L.groups < L.M ? L.groups : L.M);
+  const long long tiles = chunks * p.tiles_n;
+  if (tiles > 0x7FFFFFFFLL) return set_error(SMB_ERR_UNSUPPORTED, "i8 decode: too many tiles");
+  const int num_kb = (L.K + i8d::kBlockK - 1) / i8d::kBlockK;
+  // K split: as many CTAs per tile as SMs are free, at least two K blocks each.
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
+  p.kb_per = (num_kb + split - 1) / split;
+  split = (num_kb + p.kb_per - 1) / p.kb_per;
+  long long ctas;
+  if (split > 1) {
+    ctas = tiles * split;
+  } else {
+    // Equal shares: the CTAs that t = ceil(tiles / SMs) tiles each leave busy.
+    const long long per = (tiles + sms - 1) / sms;
+    ctas = (tiles + per - 1) / per;
+    if (L.offsets != nullptr && ctas < sms && tiles >= sms) ctas = sms;   // the bound says little about the count
+  }
+  const bool pairs = L.ldd % 2 == 0 && reinterpret_cast<uintptr_t>(L.d) % 4 == 0 && L.tma_store;
+  const int c = static_cast<int>(ctas);
+  if (L.swiglu)
+    return split > 1 ? launch_i8_decode<true, true, true>(L, p, c, split, stream)
+                     : launch_i8_decode<true, true, false>(L, p, c, split, stream);
+  if (pairs)
+    return split > 1 ? launch_i8_decode<false, true, true>(L, p, c, split, stream)
+                     : launch_i8_decode<false, true, false>(L, p, c, split, stream);
+  return split > 1 ? launch_i8_decode<false, false, true>(L, p, c, split, stream)
+                   : launch_i8_decode<false, false, false>(L, p, c, split, stream);
+}
+
+}  // namespace smb

@@ -25,12 +25,18 @@ struct I8Launch {
   const float* sb;       // scale per row of B (grouped: groups * N)
   int groups;            // 1: plain product
   const int* offsets;    // grouped: groups + 1 row offsets (device), else null
+  bool decode;           // the kernel for few rows per weight matrix (tmap boxes differ)
+  int chunk;             // decode: rows of A per tile, a multiple of 16 up to 128
+  int box_rows;          // decode: rows of A per TMA box
   bool weights_static;   // B and sb are not written by work that may still run on the stream
   int* status;
 };
 
 void i8_pick_tile(int M, int N, int K, int clusters, int* tile_n, int* sub_blocks);
 int i8_launch(const I8Launch& L, cudaStream_t stream);
+// Whether the decode kernel is taken for M rows in `groups` groups, with its chunk and box heights.
+bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows);
+int i8_decode_launch(const I8Launch& L, cudaStream_t stream);
 
 // Rows of `src` (bf16 or fp32) to int8 codes and one scale per row.  The next kernel on the stream may
 // start its prologue early.

@@ -121,7 +121,7 @@ def test_i8_pitched_output_keeps_its_padding(smb, cuda_device, m, ldd):
 
 
 @pytest.mark.parametrize("shape", [(1, 64, 48), (16, 4096, 2048), (300, 512, 256), (1030, 1552, 640), (100, 2064, 1000)])
-@pytest.mark.parametrize("tile", ["FLAG_NONE", "FLAG_TILE_N_512"])
+@pytest.mark.parametrize("tile", ["FLAG_NONE", "FLAG_TILE_N_512", "FLAG_DECODE_SINGLE"])
 def test_i8_gated_epilogue(smb, cuda_device, shape, tile):
     torch = _torch()
     m, n, k = shape
@@ -170,22 +170,23 @@ GROUPS = [((300, 0, 77, 512, 1), 384, 256), ((0, 0, 1), 130, 100), ((1,) * 40, 2
 
 
 @pytest.mark.parametrize("case", GROUPS, ids=lambda c: f"{len(c[0])}x{c[1]}x{c[2]}")
-@pytest.mark.parametrize("mode", ["plain", "gated", "no_decode", "wide", "plain_store"])
+@pytest.mark.parametrize("mode", ["plain", "gated", "no_decode", "wide", "plain_store", "decode", "decode_gated"])
 def test_i8_grouped_ragged(smb, cuda_device, case, mode):
     torch = _torch()
     sizes, n, k = case
     c = smb.capi
     flags = {"plain": 0, "gated": c.FLAG_EPILOGUE_SWIGLU, "no_decode": c.FLAG_NO_DECODE,
-             "wide": c.FLAG_NO_DECODE | c.FLAG_TILE_N_512, "plain_store": c.FLAG_FORCE_PLAIN_STORE}[mode]
-    if mode == "gated":
+             "wide": c.FLAG_NO_DECODE | c.FLAG_TILE_N_512, "plain_store": c.FLAG_FORCE_PLAIN_STORE,
+             "decode": c.FLAG_DECODE_SINGLE, "decode_gated": c.FLAG_DECODE_SINGLE | c.FLAG_EPILOGUE_SWIGLU}[mode]
+    if mode.endswith("gated"):
         n = (n + 15) // 16 * 16
     plan, ends, offsets, a, sa, b, sb, d = _run_grouped(smb, torch, sizes, n, k, flags, slack=40)
     plan.run()
     plan.check()
-    _check_grouped(torch, ends, n, k, a, sa, b, sb, d, mode == "gated")
+    _check_grouped(torch, ends, n, k, a, sa, b, sb, d, mode.endswith("gated"))
 
 
-@pytest.mark.parametrize("mode", ["FLAG_NONE", "FLAG_NO_DECODE"])
+@pytest.mark.parametrize("mode", ["FLAG_DECODE_SINGLE", "FLAG_NO_DECODE"])
 def test_i8_grouped_plan_follows_its_offsets(smb, cuda_device, mode):
     # One plan, captured once: every replay reads the offsets that are there then, the empty batch too.
     torch = _torch()
@@ -353,7 +354,7 @@ def test_i8_random_shapes_all_schedules_agree(smb, cuda_device, seed):
         m, n, k = int(rng.integers(1, 200)), int(rng.integers(1, 1500)), int(rng.integers(1, 3000))
         outs = []
         for flags in [0, c.FLAG_NO_DECODE, c.FLAG_NO_DECODE | c.FLAG_TILE_N_128, c.FLAG_NO_DECODE | c.FLAG_TILE_N_512,
-                      c.FLAG_FORCE_PLAIN_STORE, c.FLAG_WEIGHTS_STATIC]:
+                      c.FLAG_FORCE_PLAIN_STORE, c.FLAG_WEIGHTS_STATIC, c.FLAG_DECODE_SINGLE]:
             a, sa, b, sb, d = _run(smb, torch, m, n, k, flags=flags, seed=seed)
             outs.append(d)
         _check(torch, outs[0], _sums(torch, a, b, k), sa, sb)
