@@ -6,7 +6,7 @@
 // stage is mostly weights.  Accumulator lane = channel, column = token.
 //
 // One CTA per SM walks the (row chunk, channel tile) pairs; warp 0 loads (TMA), warp 1 issues the MMAs,
-// warps 2-5 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs cuts the K loop of a
+// warps 2-9 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs cuts the K loop of a
 // pair and adds its int32 partial sums through distributed shared memory: the sums are exact, so their
 // order does not matter, and there is neither workspace nor atomic.
 #include "gemm_common.cuh"
@@ -20,7 +20,8 @@ namespace i8d {
 
 constexpr int kTileRows = 128;        // channels per tile
 constexpr int kBlockK = 128;
-constexpr int kThreads = 192;
+constexpr int kThreads = 320;
+constexpr int kMaxSplit = 8;
 constexpr int kWBytes = kTileRows * kBlockK;
 constexpr int kMaxStages = 12;
 constexpr int kBarBytes = 256;
@@ -118,6 +119,10 @@ __device__ __forceinline__ Tile find_tile(const Params& p, const int* table, int
   return r;
 }
 
+__device__ __forceinline__ float token_scale(const Params& p, const Tile& tile, int c) {
+  return c < tile.rows ? p.sa[tile.row0 + c] : 0.0f;
+}
+
 // Two tokens (rows m, m + 1 of D) of this lane's channel n, already scaled.  Neighbouring lanes trade
 // halves, so that even lanes write two channels of row m and odd lanes two of row m + 1; with the gated
 // epilogue the two are up and gate of one output.
@@ -178,7 +183,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full_bar(b), 1);
-      mbar_init(acc_empty_bar(b), 4);
+      mbar_init(acc_empty_bar(b), 8);
     }
     fence_mbar_init_cluster();
   }
@@ -302,21 +307,25 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       __syncwarp();
     }
   } else {
-    // ------------------------------------------------------------- epilogue (4 warps)
+    // ------------------------------------------------------------- epilogue (8 warps)
+    // Warp quarter = the 32 lanes it may read; the two warps of a quarter take every other 16 tokens.
     const int quarter = warp & 3;
+    const int half = (warp - 2) >> 2;
     int local = 0;
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const Tile tile = find_tile(p, table, t, lane);
       const int bank = local & 1;
       const int n = tile.col0 + quarter * 32 + lane;
-      const float sb = n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
+      const float sb = !kSplit && n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
+      // Lane i holds the scale of token i of the warp's current 16.
+      float sa = !kSplit ? token_scale(p, tile, half * 16 + (lane & 15)) : 0.0f;
       if (!mbar_wait(acc_full_bar(bank), static_cast<uint32_t>(local >> 1) & 1u)) {
         if (lane == 0) report_status(p.status, kDevTimeoutEpilogue);
         break;
       }
       tc_fence_after_sync();
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(bank * p.bank_cols);
-      for (int c0 = 0; c0 < tile.rows; c0 += 16) {
+      for (int c0 = half * 16; c0 < tile.rows; c0 += 32) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(taddr + c0, v);
         tmem_ld_wait();
@@ -327,14 +336,14 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
             asm volatile("st.shared.b32 [%0], %1;" ::"r"(ring_base + ((c0 + i) * kTileRows + quarter * 32 + lane) * 4), "r"(v[i])
                          : "memory");
         } else {
+          const float scale = sa;
+          sa = token_scale(p, tile, c0 + 32 + (lane & 15));
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const int c = c0 + i;
-            if (c < tile.rows) {
-              const float s0 = p.sa[tile.row0 + c];
-              const float s1 = c + 1 < tile.rows ? p.sa[tile.row0 + c + 1] : 0.0f;
+            const float s0 = __shfl_sync(0xffffffffu, scale, i), s1 = __shfl_sync(0xffffffffu, scale, i + 1);
+            if (c < tile.rows)
               store_pair<kSwiglu, kPairs>(p, tile.row0 + c, tile.rows - c, n, scale_i32(v[i], s0, sb), scale_i32(v[i + 1], s1, sb));
-            }
           }
         }
       }
@@ -345,26 +354,39 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   }
   __syncwarp();
   if (kSplit) {
+    // CTA r of the cluster owns tokens [r * per, (r + 1) * per) of the tile; its warps take them four at a
+    // time, all partial sums of the four in flight together.
+    Tile tile = {0, 0, 0, 0};
+    if (unit < num_tiles) tile = find_tile(p, table, unit, lane);
+    const int quarter = warp & 3;
+    const int n = tile.col0 + quarter * 32 + lane;
+    const int per = ((p.chunk + split - 1) / split + 1) & ~1;
+    const int end = min(tile.rows, (rank + 1) * per);
+    float sb = 0.0f;
+    if (warp >= 2 && n < p.N && tile.rows > 0) sb = p.sb[static_cast<long long>(tile.group) * p.N + n];
     cluster_sync_all();
-    if (warp >= 2 && unit < num_tiles) {
-      // CTA r of the cluster owns tokens [r * per, (r + 1) * per) of the tile.
-      const Tile tile = find_tile(p, table, unit, lane);
-      const int quarter = warp & 3;
-      const int n = tile.col0 + quarter * 32 + lane;
-      const float sb = n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
-      const int per = ((p.chunk + split - 1) / split + 1) & ~1;
-      const int end = min(tile.rows, (rank + 1) * per);
-      for (int c = rank * per; c < end; c += 2) {
-        uint32_t a0 = 0, a1 = 0;
+    if (warp >= 2) {
+      for (int c = rank * per + ((warp - 2) >> 2) * 4; c < end; c += 8) {
+        const float sa = token_scale(p, tile, c + (lane & 3));
         const uint32_t addr = ring_base + (c * kTileRows + quarter * 32 + lane) * 4;
-        for (int q = 0; q < split; ++q) {
-          const uint32_t remote = mapa_u32(addr, q);
-          a0 += ld_shared_cluster_u32(remote);
-          a1 += ld_shared_cluster_u32(remote + kTileRows * 4);
+        uint32_t part[kMaxSplit][4];
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q) {
+          const uint32_t remote = mapa_u32(addr, q < split ? q : 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part[q][i] = q < split ? ld_shared_cluster_u32(remote + i * kTileRows * 4) : 0u;
         }
-        const float s0 = p.sa[tile.row0 + c];
-        const float s1 = c + 1 < tile.rows ? p.sa[tile.row0 + c + 1] : 0.0f;
-        store_pair<kSwiglu, kPairs>(p, tile.row0 + c, end - c, n, scale_i32(a0, s0, sb), scale_i32(a1, s1, sb));
+        uint32_t sum[4] = {};
+#pragma unroll
+        for (int q = 0; q < kMaxSplit; ++q)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] += part[q][i];
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          const float s0 = __shfl_sync(0xffffffffu, sa, i), s1 = __shfl_sync(0xffffffffu, sa, i + 1);
+          if (c + i < end)
+            store_pair<kSwiglu, kPairs>(p, tile.row0 + c + i, end - c - i, n, scale_i32(sum[i], s0, sb), scale_i32(sum[i + 1], s1, sb));
+        }
       }
     }
     cluster_sync_all();   // partial sums stay until every CTA has read them

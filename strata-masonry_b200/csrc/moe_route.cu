@@ -39,6 +39,7 @@ struct RouteParams {
   float scale;
   int* ids;
   float* weights;
+  bool wide, bias_wide;   // rows of logits / the bias start on 16-byte boundaries
 };
 
 // Bit patterns that order like the values; 0 is below every value and stands for "closed".
@@ -61,12 +62,8 @@ __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   return (static_cast<unsigned long long>(top) << 32) | low;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
-  return v;
-}
-__device__ __forceinline__ double warp_sum(double v) {
+template <class T>
+__device__ __forceinline__ T warp_sum(T v) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
   return v;
@@ -87,109 +84,114 @@ __device__ __forceinline__ float load_logit(const void* row, int e) {
   return static_cast<const float*>(row)[e];
 }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-
-// Scores p + bias of this lane's V experts (closed ones -inf); also p's largest value over the token.
-template <int V, class S>
-__device__ __forceinline__ void scores(const float (&l)[V], const float (&bias)[V], bool sigmoid, float top, S (&s)[V],
-                                       float& p_max) {
-  S sum = 0;
-  float mine = 0.0f;
+// V consecutive values from index e0 on, 0 beyond n.  kWide: the row starts on a 16-byte boundary.
+template <int V, bool kBf16>
+__device__ __forceinline__ void load_run(const void* row, int e0, int n, bool wide, float (&v)[V]) {
+  constexpr int kPer = kBf16 ? 8 : 4;   // values in 16 bytes
+  if (V % kPer == 0 && wide && e0 + V <= n) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const bool open = l[i] > -INFINITY;
-    if (sigmoid) s[i] = open ? S(1) / (S(1) + exp_of(-S(l[i]))) : S(0);
-    else s[i] = open ? exp_of(S(l[i]) - S(top)) : S(0);
-    sum += s[i];
-  }
-  if (!sigmoid) {
-    sum = warp_sum(sum);
+    for (int i = 0; i < V / kPer; ++i) {
+      const uint4 q = reinterpret_cast<const uint4*>(static_cast<const char*>(row) + e0 * (kBf16 ? 2 : 4))[i];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = sum > S(0) ? s[i] / sum : S(0);
+      for (int j = 0; j < 4; ++j) {
+        if (kBf16) {
+          v[i * kPer + 2 * j] = __uint_as_float(w[j] << 16);
+          v[i * kPer + 2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        } else {
+          v[i * kPer + j] = __uint_as_float(w[j]);
+        }
+      }
+    }
+    return;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    mine = fmaxf(mine, static_cast<float>(s[i]));
-    s[i] = l[i] > -INFINITY ? s[i] + S(bias[i]) : S(-INFINITY);
-  }
-  p_max = warp_max_float(mine);
+  for (int i = 0; i < V; ++i) v[i] = e0 + i < n ? load_logit<kBf16>(row, e0 + i) : 0.0f;
 }
 
-// Bit g set: group g stays open.  `close` is raised when the choice hangs on less than `tol` (fp32).
-template <int V, class S>
-__device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const S (&s)[V], S* buf, int lane, float p_max,
-                                                  bool& close) {
-#pragma unroll
-  for (int i = 0; i < V; ++i)
-    if (lane * V + i < p.experts) buf[lane * V + i] = s[i];
-  __syncwarp();
+// Best and second best value of a set; two sets join.
+template <class S>
+struct Top2 {
+  S best, second;
+  __device__ __forceinline__ void add(S v) {
+    second = fmax(second, fmin(best, v));
+    best = fmax(best, v);
+  }
+  __device__ __forceinline__ void join(const Top2& o) {
+    second = fmax(fmin(best, o.best), fmax(second, o.second));
+    best = fmax(best, o.best);
+  }
+  // -inf: no expert of the group is open.
+  __device__ __forceinline__ S value(bool top2) const {
+    return top2 && second > S(-INFINITY) ? best + second : best;
+  }
+};
+
+// The whole choice on fp64 scores; for the few tokens whose order hangs on the rounding of fp32.
+// `s` holds experts doubles of this warp.  Returns lane j's choice j.
+template <bool kBf16>
+__device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row, double* s, int lane) {
+  const bool sigmoid = (p.flags & SMB_ROUTE_SIGMOID) != 0;
   const int size = p.experts / p.n_groups;
-  S best = S(-INFINITY), second = S(-INFINITY);
-  if (lane < p.n_groups) {
-    for (int i = 0; i < size; ++i) {
-      const S v = buf[lane * size + i];
-      if (v > best) {
-        second = best;
-        best = v;
-      } else if (v > second) {
-        second = v;
-      }
-    }
+  float top = -INFINITY;
+  for (int e = lane; e < p.experts; e += 32) top = fmaxf(top, clean_logit(load_logit<kBf16>(row, e)));
+  top = warp_max_float(top);
+  double sum = 0.0;
+  for (int e = lane; e < p.experts; e += 32) {
+    const float l = clean_logit(load_logit<kBf16>(row, e));
+    double v = 0.0;
+    if (l > -INFINITY) v = sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(l))) : exp(static_cast<double>(l) - top);
+    s[e] = v;
+    sum += v;
+  }
+  sum = sigmoid ? 1.0 : warp_sum(sum);
+  for (int e = lane; e < p.experts; e += 32) {
+    const bool open = clean_logit(load_logit<kBf16>(row, e)) > -INFINITY;
+    const double v = s[e] / sum + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
+    s[e] = open && v > -INFINITY ? v : -INFINITY;
   }
   __syncwarp();
-  if ((p.flags & SMB_ROUTE_GROUP_TOP2) && second > S(-INFINITY)) best += second;
-  auto key = best > S(-INFINITY) ? order_key(best) : decltype(order_key(best))(0);
-  uint32_t kept = 0;
-  float prev = 0.0f;
-  for (int j = 0; j <= p.top_groups; ++j) {
-    const auto m = warp_max(key);
-    if (m == 0) break;
-    const int win = __ffs(__ballot_sync(kFull, key == m)) - 1;
-    const float value = static_cast<float>(__shfl_sync(kFull, best, win));
-    // Inside the kept set the order does not matter; only the border between kept and left out does.
-    if (j == p.top_groups) {
-      close = prev - value <= 0x1p-19f * p_max + 0x1p-21f * (fabsf(value) + fabsf(prev));
-      break;
+  uint32_t kept = kFull;
+  if (p.top_groups < p.n_groups) {
+    Top2<double> best = {-INFINITY, -INFINITY};
+    if (lane < p.n_groups)
+      for (int i = 0; i < size; ++i) best.add(s[lane * size + i]);
+    const double value = best.value((p.flags & SMB_ROUTE_GROUP_TOP2) != 0);
+    unsigned long long key = value > -INFINITY ? order_key(value) : 0ull;
+    kept = 0;
+    for (int j = 0; j < p.top_groups; ++j) {
+      const unsigned long long m = warp_max(key);
+      if (m == 0) break;
+      const int win = __ffs(__ballot_sync(kFull, key == m)) - 1;
+      kept |= 1u << win;
+      if (lane == win) key = 0;
     }
-    kept |= 1u << win;
-    if (lane == win) key = 0;
-    prev = value;
   }
-  return kept;
-}
-
-// The top_k best keys, best first: lane j ends up with the id of choice j (or -1).
-template <int V, class K>
-__device__ __forceinline__ int choose_experts(int top_k, K (&key)[V], int lane, bool check, float p_max, bool& close) {
-  int my_id = -1;
-  float prev = 0.0f;
-  for (int j = 0; j < top_k + (check ? 1 : 0); ++j) {
-    K best = key[0];
+  // Without a bias the logits are compared inside the kept groups.
+  if (p.bias == nullptr)
+    for (int e = lane; e < p.experts; e += 32) s[e] = clean_logit(load_logit<kBf16>(row, e));
+  for (int e = lane; e < p.experts; e += 32)
+    if (!((kept >> (e / size)) & 1u)) s[e] = -INFINITY;
+  __syncwarp();
+  int id = -1;
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned long long best = 0;
     int at = 0;
-#pragma unroll
-    for (int i = 1; i < V; ++i)
-      if (key[i] > best) {
-        best = key[i];
-        at = i;
+    for (int e = lane; e < p.experts; e += 32) {
+      const unsigned long long k = s[e] > -INFINITY ? order_key(s[e]) : 0ull;
+      if (k > best) {
+        best = k;
+        at = e;
       }
-    const K m = warp_max(best);
+    }
+    const unsigned long long m = warp_max(best);
     if (m == 0) break;
-    const int win = __ffs(__ballot_sync(kFull, best == m)) - 1;   // lanes hold ascending experts
-    if (check) {
-      const float value = key_value(static_cast<uint32_t>(m));
-      if (j > 0 && prev - value <= 0x1p-20f * p_max + 0x1p-22f * (fabsf(value) + fabsf(prev))) close = true;
-      prev = value;
-    }
-    const int id = __shfl_sync(kFull, lane * V + at, win);
-    if (lane == j && j < top_k) my_id = id;
-    if (lane == win) {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i == at) key[i] = 0;
-    }
+    const int e = __reduce_min_sync(kFull, best == m ? at : 0x7FFFFFFF);
+    if (lane == j) id = e;
+    if (lane == (e & 31)) s[e] = -INFINITY;
+    __syncwarp();
   }
-  return my_id;
+  return id;
 }
 
 template <int V, bool kBf16>
@@ -203,54 +205,141 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p)
   const void* row = static_cast<const char*>(p.logits) + static_cast<int64_t>(t) * p.ld * (kBf16 ? 2 : 4);
   const bool sigmoid = (p.flags & SMB_ROUTE_SIGMOID) != 0;
   const bool renorm = (p.flags & SMB_ROUTE_RENORM) != 0;
-  float l[V], bias[V];
+  const bool by_group = p.top_groups < p.n_groups;
+  const bool by_score = p.bias != nullptr;
+  const int e0 = lane * V;   // lanes hold runs of V experts, so lower lanes hold lower indices
+  float l[V];
+  load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    l[i] = e < p.experts ? clean_logit(load_logit<kBf16>(row, e)) : -INFINITY;
-    bias[i] = (p.bias != nullptr && e < p.experts) ? p.bias[e] : 0.0f;
+    l[i] = e0 + i < p.experts ? clean_logit(l[i]) : -INFINITY;
     top = fmaxf(top, l[i]);
   }
-  top = warp_max_float(top);
-  const bool by_group = p.top_groups < p.n_groups;
-  const bool by_score = p.bias != nullptr;
+  if (!sigmoid) top = warp_max_float(top);
 
-  float s[V];
-  float p_max = 0.0f;
-  if (by_score || by_group) scores<V, float>(l, bias, sigmoid, top, s, p_max);
-  uint32_t kept = kFull;
-  if (by_group) {
-    bool close = false;
-    kept = choose_groups<V, float>(p, s, reinterpret_cast<float*>(buf_all[warp]), lane, p_max, close);
-    if (close) {
-      double d[V];
-      float unused;
-      scores<V, double>(l, bias, sigmoid, top, d, unused);
-      kept = choose_groups<V, double>(p, d, buf_all[warp], lane, p_max, close);
-    }
-  }
-  const int size = p.experts / p.n_groups;
-  auto open = [&](int i) {
-    return l[i] > -INFINITY && (!by_group || ((kept >> ((lane * V + i) / size)) & 1u));
-  };
   uint32_t key[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float v = by_score ? s[i] : l[i];
-    key[i] = open(i) && v > -INFINITY ? order_key(v) : 0u;   // a bias of -inf closes an expert too
-  }
+  float p_max = 0.0f;
   bool close = false;
-  int id = choose_experts<V, uint32_t>(p.top_k, key, lane, by_score, p_max, close);
-  if (close) {
-    double d[V];
-    float unused;
-    scores<V, double>(l, bias, sigmoid, top, d, unused);
-    unsigned long long wide[V];
+  if (by_score || by_group) {
+    float s[V];
+    float sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) wide[i] = open(i) && d[i] > -INFINITY ? order_key(d[i]) : 0ull;
-    id = choose_experts<V, unsigned long long>(p.top_k, wide, lane, false, p_max, close);
+    for (int i = 0; i < V; ++i) {
+      // expf of -inf is 0 and of +inf infinity: closed experts come out as p = 0 in both forms.
+      s[i] = sigmoid ? __fdividef(1.0f, 1.0f + expf(-l[i])) : (l[i] > -INFINITY ? expf(l[i] - top) : 0.0f);
+      sum += s[i];
+    }
+    if (!sigmoid) {
+      sum = warp_sum(sum);
+      const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) p_max = fmaxf(p_max, s[i]);
+    p_max = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(p_max)));   // p >= 0: bits order as they are
+    if (by_score) {
+      float b[V];
+      load_run<V, false>(p.bias, e0, p.experts, p.bias_wide, b);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += b[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = l[i] > -INFINITY && s[i] > -INFINITY ? s[i] : -INFINITY;
+    uint32_t kept = kFull;
+    const int size = p.experts / p.n_groups;
+    if (by_group) {
+      Top2<float> best = {-INFINITY, -INFINITY};
+      float value;
+      int group = lane;   // whose value this lane holds
+      const int lanes = size / V;
+      if (lanes * V == size && (lanes & (lanes - 1)) == 0) {
+        // A group is a run of 2^n whole lanes: join them by shuffles; its first lane speaks for it.
+#pragma unroll
+        for (int i = 0; i < V; ++i) best.add(s[i]);
+        for (int d = 1; d < lanes; d <<= 1) {
+          const Top2<float> o = {__shfl_xor_sync(kFull, best.best, d), __shfl_xor_sync(kFull, best.second, d)};
+          best.join(o);
+        }
+        group = lane / lanes;
+        value = (lane & (lanes - 1)) == 0 && group < p.n_groups ? best.value((p.flags & SMB_ROUTE_GROUP_TOP2) != 0) : -INFINITY;
+      } else {
+        float* buf = reinterpret_cast<float*>(buf_all[warp]);   // padded: a word after every 32
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (e0 + i < p.experts) buf[e0 + i + ((e0 + i) >> 5)] = s[i];
+        __syncwarp();
+        if (lane < p.n_groups)
+          for (int i = 0; i < size; ++i) best.add(buf[lane * size + i + ((lane * size + i) >> 5)]);
+        __syncwarp();
+        value = lane < p.n_groups ? best.value((p.flags & SMB_ROUTE_GROUP_TOP2) != 0) : -INFINITY;
+      }
+      uint32_t gkey = value > -INFINITY ? order_key(value) : 0u;
+      kept = 0;
+      float prev = 0.0f;
+      for (int j = 0; j <= p.top_groups; ++j) {
+        const uint32_t m = __reduce_max_sync(kFull, gkey);
+        if (m == 0) break;
+        const float v = key_value(m);
+        // Inside the kept set the order does not matter, only the border to what is left out.
+        if (j == p.top_groups) {
+          close = prev - v <= 0x1p-19f * p_max + 0x1p-21f * (fabsf(v) + fabsf(prev));
+          break;
+        }
+        const int win = __ffs(__ballot_sync(kFull, gkey == m)) - 1;
+        kept |= 1u << __shfl_sync(kFull, group, win);
+        if (lane == win) gkey = 0;
+        prev = v;
+      }
+    }
+    int g = e0 / size, in_group = e0 - g * size;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float v = by_score ? s[i] : l[i];
+      const bool open = s[i] > -INFINITY && ((kept >> (g & 31)) & 1u);   // a bias of -inf closes an expert too
+      key[i] = open ? order_key(v) : 0u;
+      if (++in_group == size) {
+        in_group = 0;
+        ++g;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = l[i] > -INFINITY ? order_key(l[i]) : 0u;
   }
+
+  int id = -1;
+  if (!close) {
+    float prev = 0.0f;
+    const int rounds = p.top_k + (by_score ? 1 : 0);   // one more to see what the last choice won against
+    for (int j = 0; j < rounds; ++j) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i]);
+      const uint32_t m = __reduce_max_sync(kFull, best);
+      if (m == 0) break;
+      if (by_score) {
+        const float v = key_value(m);
+        if (j > 0 && prev - v <= 0x1p-20f * p_max + 0x1p-22f * (fabsf(v) + fabsf(prev))) {
+          close = true;
+          break;
+        }
+        prev = v;
+      }
+      const int win = __ffs(__ballot_sync(kFull, best == m)) - 1;
+      int at = 0;
+#pragma unroll
+      for (int i = V - 1; i >= 0; --i) at = key[i] == m ? i : at;
+      const int e = __shfl_sync(kFull, e0 + at, win);
+      if (lane == j) id = e;
+      at = lane == win ? at : -1;
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
+    }
+    if (lane >= p.top_k) id = -1;
+  }
+  if (close) id = choose_in_fp64<kBf16>(p, row, buf_all[warp], lane);
 
   // Weights: lane j has choice j.
   const float lj = id >= 0 ? clean_logit(load_logit<kBf16>(row, id)) : -INFINITY;
@@ -294,6 +383,7 @@ struct RouteGradParams {
   float scale;
   void* grad_logits;
   int64_t ld_grad;
+  bool wide, grad_wide, grad_even;   // 16-byte rows of logits and gradient, 4-byte rows of the gradient
 };
 
 template <int V, bool kBf16>
@@ -315,14 +405,15 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteGrad
   }
   const bool has = lj > -INFINITY;
   // Softmax over all experts is needed only where its sum is the denominator.
+  const int e0 = lane * V;
   float l[V], top = -INFINITY, inv_sum = 0.0f;
   const bool dense = !sigmoid && !renorm;
   if (dense) {
     float sum = 0.0f;
+    load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const int e = lane * V + i;
-      l[i] = e < p.experts ? clean_logit(load_logit<kBf16>(row, e)) : -INFINITY;
+      l[i] = e0 + i < p.experts ? clean_logit(l[i]) : -INFINITY;
       top = fmaxf(top, l[i]);
     }
     top = warp_max_float(top);
@@ -370,18 +461,36 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteGrad
     const float v = __shfl_sync(kFull, part, j);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (lane * V + i == e) out[i] += v;
+      if (e0 + i == e) out[i] += v;
+  }
+  char* dst = static_cast<char*>(p.grad_logits) + static_cast<int64_t>(t) * p.ld_grad * (kBf16 ? 2 : 4);
+  constexpr int kPer = kBf16 ? 8 : 4;
+  if (V % kPer == 0 && p.grad_wide && e0 + V <= p.experts) {
+#pragma unroll
+    for (int i = 0; i < V; i += kPer) {
+      uint4 q;
+      if (kBf16) {
+        q.x = pack_bf16x2(__float_as_uint(out[i]), __float_as_uint(out[(i + 1) % V]));
+        q.y = pack_bf16x2(__float_as_uint(out[(i + 2) % V]), __float_as_uint(out[(i + 3) % V]));
+        q.z = pack_bf16x2(__float_as_uint(out[(i + 4) % V]), __float_as_uint(out[(i + 5) % V]));
+        q.w = pack_bf16x2(__float_as_uint(out[(i + 6) % V]), __float_as_uint(out[(i + 7) % V]));
+      } else {
+        q = make_uint4(__float_as_uint(out[i]), __float_as_uint(out[(i + 1) % V]), __float_as_uint(out[(i + 2) % V]),
+                       __float_as_uint(out[(i + 3) % V]));
+      }
+      *reinterpret_cast<uint4*>(dst + (e0 + i) * (kBf16 ? 2 : 4)) = q;
+    }
+    return;
+  }
+  if (V == 2 && kBf16 && p.grad_even && e0 + 2 <= p.experts) {
+    *reinterpret_cast<uint32_t*>(dst + e0 * 2) = pack_bf16x2(__float_as_uint(out[0]), __float_as_uint(out[V - 1]));
+    return;
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const int e = lane * V + i;
-    if (e >= p.experts) continue;
-    if (kBf16) {
-      static_cast<uint16_t*>(p.grad_logits)[static_cast<int64_t>(t) * p.ld_grad + e] =
-          static_cast<uint16_t>(pack_bf16x2(__float_as_uint(out[i]), 0u) & 0xFFFFu);
-    } else {
-      static_cast<float*>(p.grad_logits)[static_cast<int64_t>(t) * p.ld_grad + e] = out[i];
-    }
+    if (e0 + i >= p.experts) continue;
+    if (kBf16) reinterpret_cast<uint16_t*>(dst)[e0 + i] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(out[i]), 0u) & 0xFFFFu);
+    else reinterpret_cast<float*>(dst)[e0 + i] = out[i];
   }
 }
 
@@ -461,7 +570,10 @@ extern "C" int smb_moe_route_device(const void* logits, int dtype, int64_t ld, c
     return set_error(SMB_ERR_INVALID, "route: top_k=%d above the %d experts of the open groups", top_k,
                      experts / n_groups * top_groups);
   if (tokens == 0) return SMB_OK;
-  const RouteParams p = {logits, ld, bias, tokens, experts, top_k, n_groups, top_groups, flags, scale, ids, weights};
+  const int size = dtype == SMB_DTYPE_BF16 ? 2 : 4;
+  const bool wide = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld * size) % 16 == 0;
+  const RouteParams p = {logits, ld,    bias, tokens,  experts, top_k, n_groups, top_groups,
+                         flags,  scale, ids,  weights, wide,    reinterpret_cast<uintptr_t>(bias) % 16 == 0};
   return by_width<LaunchRoute>(dtype == SMB_DTYPE_BF16, experts, p, static_cast<cudaStream_t>(stream));
 }
 
@@ -477,6 +589,10 @@ extern "C" int smb_moe_route_backward_device(const void* logits, int dtype, int6
   if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == SMB_DTYPE_BF16 ? 2 : 4) != 0)
     return set_error(SMB_ERR_INVALID, "route backward: gradient is not aligned to its type");
   if (tokens == 0) return SMB_OK;
-  const RouteGradParams p = {logits, ld, ids, grad_weights, tokens, experts, top_k, flags, scale, grad_logits, ld_grad};
+  const int size = dtype == SMB_DTYPE_BF16 ? 2 : 4;
+  auto rows_at = [](const void* q, int64_t bytes, int n) { return reinterpret_cast<uintptr_t>(q) % n == 0 && bytes % n == 0; };
+  const RouteGradParams p = {logits, ld, ids, grad_weights, tokens, experts, top_k, flags, scale, grad_logits, ld_grad,
+                             rows_at(logits, ld * size, 16), rows_at(grad_logits, ld_grad * size, 16),
+                             rows_at(grad_logits, ld_grad * size, 4)};
   return by_width<LaunchRouteGrad>(dtype == SMB_DTYPE_BF16, experts, p, static_cast<cudaStream_t>(stream));
 }
