@@ -40,13 +40,16 @@ struct RouteParams {
   int* ids;
   float* weights;
   bool wide, bias_wide;   // rows of logits / the bias start on 16-byte boundaries
+  int group_size;         // experts per group
+  int group_lanes;        // lanes per group where that is a power of two of whole lanes, else 0
 };
 
-// Bit patterns that order like the values; 0 is below every value and stands for "closed".
+// Bit patterns that order like the values.  Keys up to that of -inf stand for "closed".
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
-  return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  return b ^ (static_cast<uint32_t>(static_cast<int>(b) >> 31) | 0x80000000u);
 }
+constexpr uint32_t kClosedKey = 0x007FFFFFu;
 __device__ __forceinline__ unsigned long long order_key(double v) {
   const unsigned long long b = static_cast<unsigned long long>(__double_as_longlong(v));
   return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
@@ -72,11 +75,19 @@ __device__ __forceinline__ float warp_max_float(float v) {
   return key_value(__reduce_max_sync(kFull, order_key(v)));
 }
 
-// Logits as this file uses them: closed experts are -inf, +inf is the largest finite value.
-__device__ __forceinline__ float clean_logit(float l) {
-  if (!(l > -INFINITY)) return -INFINITY;
-  return fminf(l, FLT_MAX);
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Logits as this file uses them: closed experts are -inf, +inf is the largest finite value.
+__device__ __forceinline__ float clean_logit(float l) { return fminf(fmaxf(l, -INFINITY), FLT_MAX); }
 
 template <bool kBf16>
 __device__ __forceinline__ float load_logit(const void* row, int e) {
@@ -84,7 +95,7 @@ __device__ __forceinline__ float load_logit(const void* row, int e) {
   return static_cast<const float*>(row)[e];
 }
 
-// V consecutive values from index e0 on, 0 beyond n.  kWide: the row starts on a 16-byte boundary.
+// V consecutive values from index e0 on, -inf beyond n.  `wide`: the row starts on a 16-byte boundary.
 template <int V, bool kBf16>
 __device__ __forceinline__ void load_run(const void* row, int e0, int n, bool wide, float (&v)[V]) {
   constexpr int kPer = kBf16 ? 8 : 4;   // values in 16 bytes
@@ -106,7 +117,7 @@ __device__ __forceinline__ void load_run(const void* row, int e0, int n, bool wi
     return;
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = e0 + i < n ? load_logit<kBf16>(row, e0 + i) : 0.0f;
+  for (int i = 0; i < V; ++i) v[i] = e0 + i < n ? load_logit<kBf16>(row, e0 + i) : -INFINITY;
 }
 
 // Best and second best value of a set; two sets join.
@@ -194,8 +205,34 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
   return id;
 }
 
+// Batcher's odd-even merge sort, largest first.
+template <int V>
+__device__ __forceinline__ void sort_down(uint32_t (&k)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int lo = 0; lo < V; ++lo) {
+        const int hi = lo + q;
+        // q == p merges runs from their first elements on, smaller q the inner ones.
+        const bool used = hi < V && lo / (2 * p) == hi / (2 * p) && (lo >= q % p) && ((lo - q % p) / q) % 2 == 0;
+        if (used) {
+          const uint32_t x = k[lo], y = k[hi];
+          k[lo] = max(x, y);
+          k[hi] = min(x, y);
+        }
+      }
+}
+
+// What bounds it: instructions.  A token of 256 experts is 1 KB to read (0.16 ns at the copy rate), but
+// eight choices out of it are hundreds of warp instructions, most of them on the half-rate ALU pipe.  So
+// every lane sorts its V scores once, with the position inside the lane in the low bits of the key (two
+// instructions per compare-exchange), and a choice is then one redux, one ballot and a shift of the
+// winner's list.  The bits that the position covers are made good like the rounding of exp: neighbours
+// closer than their worth go to the fp64 choice.
 template <int V, bool kBf16>
-__global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(const RouteParams p) {
   __shared__ double buf_all[kWarps][kMaxExperts];
   griddep_launch_dependents();
   griddep_wait();
@@ -207,32 +244,42 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p)
   const bool renorm = (p.flags & SMB_ROUTE_RENORM) != 0;
   const bool by_group = p.top_groups < p.n_groups;
   const bool by_score = p.bias != nullptr;
+  const bool exact = kBf16 && !by_score;   // bf16 logits leave the low 16 bits of the key free
+  constexpr uint32_t kPos = V <= 1 ? 0 : (V <= 2 ? 1 : (V <= 4 ? 3 : (V <= 8 ? 7 : 15)));
   const int e0 = lane * V;   // lanes hold runs of V experts, so lower lanes hold lower indices
   float l[V];
   load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
-  float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    l[i] = e0 + i < p.experts ? clean_logit(l[i]) : -INFINITY;
-    top = fmaxf(top, l[i]);
+  for (int i = 0; i < V; ++i) l[i] = clean_logit(l[i]);
+  float top = 0.0f;
+  if (!sigmoid) {
+    top = l[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) top = fmaxf(top, l[i]);
+    top = warp_max_float(top);
   }
-  if (!sigmoid) top = warp_max_float(top);
 
   uint32_t key[V];
   float p_max = 0.0f;
   bool close = false;
   if (by_score || by_group) {
     float s[V];
-    float sum = 0.0f;
+    constexpr float kLog2e = 1.4426950408889634f;
+    // exp as one product and ex2.approx: off by (2 + 1.2 |l|) steps of 2^-24 relative, which the
+    // thresholds below allow for (2^-16 of the largest p for two scores).
+    if (sigmoid) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      // expf of -inf is 0 and of +inf infinity: closed experts come out as p = 0 in both forms.
-      s[i] = sigmoid ? __fdividef(1.0f, 1.0f + expf(-l[i])) : (l[i] > -INFINITY ? expf(l[i] - top) : 0.0f);
-      sum += s[i];
-    }
-    if (!sigmoid) {
+      for (int i = 0; i < V; ++i) s[i] = rcp_approx(1.0f + ex2_approx(-l[i] * kLog2e));   // closed: 1 / (1 + inf) = 0
+    } else {
+      float sum = 0.0f;
+      const float shift = fmaxf(top, -FLT_MAX);   // no open expert at all: (-inf) - (-FLT_MAX) gives 0
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        s[i] = ex2_approx((l[i] - shift) * kLog2e);
+        sum += s[i];
+      }
       sum = warp_sum(sum);
-      const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+      const float inv = sum > 0.0f ? rcp_approx(sum) : 0.0f;
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] *= inv;
     }
@@ -246,24 +293,24 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p)
       for (int i = 0; i < V; ++i) s[i] += b[i];
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = l[i] > -INFINITY && s[i] > -INFINITY ? s[i] : -INFINITY;
-    uint32_t kept = kFull;
-    const int size = p.experts / p.n_groups;
+    for (int i = 0; i < V; ++i) {
+      s[i] = l[i] > -INFINITY ? fmaxf(s[i], -INFINITY) : -INFINITY;   // a bias of -inf or NaN closes an expert too
+      key[i] = (order_key(by_score ? s[i] : l[i]) & ~kPos) | (kPos - i);
+    }
     if (by_group) {
       Top2<float> best = {-INFINITY, -INFINITY};
-      float value;
-      int group = lane;   // whose value this lane holds
-      const int lanes = size / V;
-      if (lanes * V == size && (lanes & (lanes - 1)) == 0) {
-        // A group is a run of 2^n whole lanes: join them by shuffles; its first lane speaks for it.
+      const bool top2 = (p.flags & SMB_ROUTE_GROUP_TOP2) != 0;
+      float value = -INFINITY;   // lane g: value of group g
+      const int lanes = p.group_lanes;
+      if (lanes != 0) {
+        // A group is a run of 2^n whole lanes: join them by shuffles.
 #pragma unroll
         for (int i = 0; i < V; ++i) best.add(s[i]);
         for (int d = 1; d < lanes; d <<= 1) {
           const Top2<float> o = {__shfl_xor_sync(kFull, best.best, d), __shfl_xor_sync(kFull, best.second, d)};
           best.join(o);
         }
-        group = lane / lanes;
-        value = (lane & (lanes - 1)) == 0 && group < p.n_groups ? best.value((p.flags & SMB_ROUTE_GROUP_TOP2) != 0) : -INFINITY;
+        value = __shfl_sync(kFull, best.value(top2), lane * lanes);
       } else {
         float* buf = reinterpret_cast<float*>(buf_all[warp]);   // padded: a word after every 32
 #pragma unroll
@@ -271,73 +318,81 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p)
           if (e0 + i < p.experts) buf[e0 + i + ((e0 + i) >> 5)] = s[i];
         __syncwarp();
         if (lane < p.n_groups)
-          for (int i = 0; i < size; ++i) best.add(buf[lane * size + i + ((lane * size + i) >> 5)]);
+          for (int i = 0; i < p.group_size; ++i) best.add(buf[lane * p.group_size + i + ((lane * p.group_size + i) >> 5)]);
         __syncwarp();
-        value = lane < p.n_groups ? best.value((p.flags & SMB_ROUTE_GROUP_TOP2) != 0) : -INFINITY;
+        value = best.value(top2);
       }
-      uint32_t gkey = value > -INFINITY ? order_key(value) : 0u;
-      kept = 0;
-      float prev = 0.0f;
-      for (int j = 0; j <= p.top_groups; ++j) {
-        const uint32_t m = __reduce_max_sync(kFull, gkey);
-        if (m == 0) break;
-        const float v = key_value(m);
-        // Inside the kept set the order does not matter, only the border to what is left out.
-        if (j == p.top_groups) {
-          close = prev - v <= 0x1p-19f * p_max + 0x1p-21f * (fabsf(v) + fabsf(prev));
-          break;
-        }
-        const int win = __ffs(__ballot_sync(kFull, gkey == m)) - 1;
-        kept |= 1u << __shfl_sync(kFull, group, win);
-        if (lane == win) gkey = 0;
-        prev = v;
+      const uint32_t gkey = lane < p.n_groups ? order_key(value) : 0u;
+      // A group stays open if fewer than top_groups come before it (higher value, or equal and lower index).
+      int ahead = 0;
+      for (int g = 0; g < p.n_groups; ++g) {
+        const uint32_t other = __shfl_sync(kFull, gkey, g);
+        ahead += other > gkey || (other == gkey && g < lane) ? 1 : 0;
       }
-    }
-    int g = e0 / size, in_group = e0 - g * size;
+      const bool in = lane < p.n_groups && ahead < p.top_groups;
+      const uint32_t kept = __ballot_sync(kFull, in);
+      // Only the border matters: the last group kept against the first left out.
+      const uint32_t last = __reduce_min_sync(kFull, in ? gkey : 0xFFFFFFFFu);
+      const uint32_t first = __reduce_max_sync(kFull, in ? 0u : gkey);
+      if (first > kClosedKey) {
+        const float v = key_value(last), w = key_value(first);
+        close = v - w <= 0x1p-15f * p_max + 0x1p-21f * (fabsf(v) + fabsf(w));
+      }
+      if (lanes != 0) {
+        const bool closed = !((kept >> ((lane >> (31 - __clz(lanes))) & 31)) & 1u);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float v = by_score ? s[i] : l[i];
-      const bool open = s[i] > -INFINITY && ((kept >> (g & 31)) & 1u);   // a bias of -inf closes an expert too
-      key[i] = open ? order_key(v) : 0u;
-      if (++in_group == size) {
-        in_group = 0;
-        ++g;
+        for (int i = 0; i < V; ++i) key[i] = closed ? 0u : key[i];
+      } else {
+        int g = e0 / p.group_size, in_group = e0 - g * p.group_size;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          key[i] = ((kept >> (g & 31)) & 1u) ? key[i] : 0u;
+          if (++in_group == p.group_size) {
+            in_group = 0;
+            ++g;
+          }
+        }
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = l[i] > -INFINITY ? order_key(l[i]) : 0u;
+    for (int i = 0; i < V; ++i) key[i] = (order_key(l[i]) & ~kPos) | (kPos - i);
   }
 
   int id = -1;
   if (!close) {
-    float prev = 0.0f;
-    const int rounds = p.top_k + (by_score ? 1 : 0);   // one more to see what the last choice won against
-    for (int j = 0; j < rounds; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) best = max(best, key[i]);
-      const uint32_t m = __reduce_max_sync(kFull, best);
-      if (m == 0) break;
-      if (by_score) {
-        const float v = key_value(m);
-        if (j > 0 && prev - v <= 0x1p-20f * p_max + 0x1p-22f * (fabsf(v) + fabsf(prev))) {
-          close = true;
-          break;
-        }
-        prev = v;
+    sort_down<V>(key);
+    uint32_t mine = 0;   // lane j: key and lane of choice j
+    int from = 0;
+    uint32_t border = 0;
+    for (int j = 0; j < p.top_k; ++j) {
+      const uint32_t head = key[0] & ~kPos;
+      const uint32_t m = __reduce_max_sync(kFull, head);
+      if (m <= kClosedKey) break;
+      const int win = __ffs(__ballot_sync(kFull, head == m)) - 1;   // lanes hold ascending experts
+      const uint32_t k = __shfl_sync(kFull, key[0], win);
+      if (lane == j) {
+        mine = k;
+        from = win;
       }
-      const int win = __ffs(__ballot_sync(kFull, best == m)) - 1;
-      int at = 0;
+      const bool pop = lane == win;
 #pragma unroll
-      for (int i = V - 1; i >= 0; --i) at = key[i] == m ? i : at;
-      const int e = __shfl_sync(kFull, e0 + at, win);
-      if (lane == j) id = e;
-      at = lane == win ? at : -1;
-#pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = i == at ? 0u : key[i];
+      for (int i = 0; i + 1 < V; ++i) key[i] = pop ? key[i + 1] : key[i];
+      key[V - 1] = pop ? 0u : key[V - 1];
     }
-    if (lane >= p.top_k) id = -1;
+    if (!exact) {
+      border = __reduce_max_sync(kFull, key[0] & ~kPos);   // what the last choice won against
+      const uint32_t have = mine & ~kPos;
+      uint32_t next = __shfl_down_sync(kFull, have, 1);
+      if (lane == p.top_k - 1) next = border;
+      bool tie = have == next;
+      if (by_score) {
+        const float v = key_value(have), w = key_value(next);
+        tie = v - w <= 0x1p-16f * p_max + 0x1p-19f * (fabsf(v) + fabsf(w));
+      }
+      close = __any_sync(kFull, tie && lane < p.top_k && have > kClosedKey && next > kClosedKey);
+    }
+    if (mine != 0) id = from * V + static_cast<int>(kPos - (mine & kPos));
   }
   if (close) id = choose_in_fp64<kBf16>(p, row, buf_all[warp], lane);
 
@@ -347,20 +402,21 @@ __global__ void __launch_bounds__(kWarps * 32) route_kernel(const RouteParams p)
   if (sigmoid) {
     const float low = fminf(lj, 0.0f);
     const float ref = renorm ? warp_max_float(low) : 0.0f;
-    if (id >= 0) w = expf(low - ref) / (1.0f + expf(-fabsf(lj)));
+    if (id >= 0) w = __fdividef(expf(low - ref), 1.0f + expf(-fabsf(lj)));
   } else if (renorm) {
     const float ref = warp_max_float(lj);
     if (id >= 0) w = expf(lj - ref);
   } else {
     float sum = 0.0f;
+    load_run<V, kBf16>(row, e0, p.experts, p.wide, l);   // again, so that nothing holds it meanwhile
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum += l[i] > -INFINITY ? expf(l[i] - top) : 0.0f;
+    for (int i = 0; i < V; ++i) sum += l[i] > -INFINITY ? expf(clean_logit(l[i]) - top) : 0.0f;
     sum = warp_sum(sum);
-    if (id >= 0) w = expf(lj - top) / sum;
+    if (id >= 0) w = __fdividef(expf(lj - top), sum);
   }
   if (renorm) {
-    const float sum = warp_sum(w);
-    w = id >= 0 ? w / sum : 0.0f;
+    const float sum = warp_sum(w);   // at least the largest choice's own 1 or 1/2
+    w = id >= 0 ? __fdividef(w, sum) : 0.0f;
   }
   if (lane < p.top_k) {
     p.ids[static_cast<int64_t>(t) * p.top_k + lane] = id;
@@ -413,7 +469,7 @@ __global__ void __launch_bounds__(kWarps * 32) route_grad_kernel(const RouteGrad
     load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      l[i] = e0 + i < p.experts ? clean_logit(l[i]) : -INFINITY;
+      l[i] = clean_logit(l[i]);
       top = fmaxf(top, l[i]);
     }
     top = warp_max_float(top);
@@ -540,7 +596,11 @@ int by_width(bool bf16, int experts, const P& p, cudaStream_t st) {
 
 template <int V, bool kBf16>
 struct LaunchRoute {
-  static int go(const RouteParams& p, cudaStream_t st) { return launch_tokens(route_kernel<V, kBf16>, p, st, "route launch"); }
+  static int go(RouteParams p, cudaStream_t st) {
+    const int lanes = p.group_size / V;
+    p.group_lanes = lanes * V == p.group_size && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+    return launch_tokens(route_kernel<V, kBf16>, p, st, "route launch");
+  }
 };
 template <int V, bool kBf16>
 struct LaunchRouteGrad {
@@ -573,7 +633,8 @@ extern "C" int smb_moe_route_device(const void* logits, int dtype, int64_t ld, c
   const int size = dtype == SMB_DTYPE_BF16 ? 2 : 4;
   const bool wide = reinterpret_cast<uintptr_t>(logits) % 16 == 0 && (ld * size) % 16 == 0;
   const RouteParams p = {logits, ld,    bias, tokens,  experts, top_k, n_groups, top_groups,
-                         flags,  scale, ids,  weights, wide,    reinterpret_cast<uintptr_t>(bias) % 16 == 0};
+                         flags,  scale, ids,  weights, wide,    reinterpret_cast<uintptr_t>(bias) % 16 == 0,
+                         experts / n_groups, 0};
   return by_width<LaunchRoute>(dtype == SMB_DTYPE_BF16, experts, p, static_cast<cudaStream_t>(stream));
 }
 
