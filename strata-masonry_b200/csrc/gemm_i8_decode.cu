@@ -445,10 +445,12 @@ bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int
     *box_rows = *chunk;
     return true;
   }
+  // Chunks of twice the average, so that few experts need two; above 96 rows per expert the 256-row
+  // tiles win.  64 experts of 2048 x 2048, us here (chunk) / tiled: 8 rows each 47.0 (16) / 56.1, 24 46.6
+  // (64) / 58.4, 48 47.6 (64) / 59.8, 95 55.8 (128) / 60.2, 127 75.1 (128) / 61.8.
   const int average = (M + groups - 1) / groups;
-  if (average > 32 && !force) return false;
-  *chunk = average <= 8 ? 16 : (average <= 16 ? 32 : 64);
-  if (average > 64) *chunk = 128;
+  if (average > 96 && !force) return false;
+  *chunk = average <= 8 ? 16 : (average <= 16 ? 32 : (average <= 48 ? 64 : 128));
   *box_rows = 16;
   return true;
 }

@@ -11,8 +11,8 @@
 // id -1 and weight 0, so a padding row of -inf logits goes nowhere.
 //
 // Scores are fp32.  Where two neighbours in the order (or the last chosen and the first left out) lie
-// closer together than the fp32 error of p, the warp repeats the choice on fp64 scores, so the ids are
-// those of the exact scores whatever exp rounds to.  Choices on logits need no such care.
+// closer together than the fp32 error of p, fp64 scores of the experts in question decide, so the ids
+// are those of the exact scores whatever exp rounds to.  Choices on bf16 logits need no such care.
 //
 // Renormalised weights are formed from exponentials relative to the largest chosen one, so tiny
 // probabilities do not underflow before they are divided.
@@ -138,7 +138,8 @@ struct Top2 {
   }
 };
 
-// The whole choice on fp64 scores; for the few tokens whose order hangs on the rounding of fp32.
+// The whole choice on fp64 scores: for tokens whose groups, or more experts than a warp has lanes, lie
+// closer together than fp32 can tell.
 // `s` holds experts doubles of this warp.  Returns lane j's choice j.
 template <bool kBf16>
 __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row, double* s, int lane) {
@@ -203,6 +204,47 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
     __syncwarp();
   }
   return id;
+}
+
+// Lanes 0 .. n - 1 hold the ids of all experts that can be among the top_k; their fp64 scores (logits
+// without a bias) settle the order.  Returns lane j's choice j.
+template <bool kBf16>
+__device__ __noinline__ int order_in_fp64(const RouteParams& p, const void* row, int id, int n, int lane) {
+  const bool sigmoid = (p.flags & SMB_ROUTE_SIGMOID) != 0;
+  const float l = id >= 0 ? clean_logit(load_logit<kBf16>(row, id)) : -INFINITY;
+  double score = l;
+  if (p.bias != nullptr) {
+    double sum = 1.0, top = 0.0;
+    if (!sigmoid) {
+      float m = -INFINITY;
+      for (int e = lane; e < p.experts; e += 32) m = fmaxf(m, clean_logit(load_logit<kBf16>(row, e)));
+      top = warp_max_float(m);
+      sum = 0.0;
+#pragma unroll 4
+      for (int e = lane; e < p.experts; e += 32) {
+        const float v = clean_logit(load_logit<kBf16>(row, e));
+        sum += v > -INFINITY ? exp(static_cast<double>(v) - top) : 0.0;
+      }
+      sum = warp_sum(sum);
+    }
+    if (id >= 0) {
+      const double e = exp(sigmoid ? -score : score - top);
+      score = (sigmoid ? 1.0 / (1.0 + e) : e / sum) + static_cast<double>(p.bias[id]);
+    }
+  }
+  int rank = 0;
+  for (int c = 0; c < n; ++c) {
+    const double other = __shfl_sync(kFull, score, c);
+    const int other_id = __shfl_sync(kFull, id, c);
+    rank += other > score || (other == score && other_id < id) ? 1 : 0;
+  }
+  if (lane >= n) rank = 32;
+  int out = -1;
+  for (int c = 0; c < n; ++c) {
+    const int r = __shfl_sync(kFull, rank, c), other_id = __shfl_sync(kFull, id, c);
+    if (r == lane) out = other_id;
+  }
+  return lane < p.top_k ? out : -1;
 }
 
 // Batcher's odd-even merge sort, largest first.
@@ -362,14 +404,10 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
   int id = -1;
   if (!close) {
     sort_down<V>(key);
-    uint32_t mine = 0;   // lane j: key and lane of choice j
+    uint32_t mine = 0;   // lane j: key and lane of the j-th best
     int from = 0;
-    uint32_t border = 0;
-    for (int j = 0; j < p.top_k; ++j) {
-      const uint32_t head = key[0] & ~kPos;
-      const uint32_t m = __reduce_max_sync(kFull, head);
-      if (m <= kClosedKey) break;
-      const int win = __ffs(__ballot_sync(kFull, head == m)) - 1;   // lanes hold ascending experts
+    auto take = [&](int j, uint32_t m) {
+      const int win = __ffs(__ballot_sync(kFull, (key[0] & ~kPos) == m)) - 1;   // lanes hold ascending experts
       const uint32_t k = __shfl_sync(kFull, key[0], win);
       if (lane == j) {
         mine = k;
@@ -379,18 +417,37 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
 #pragma unroll
       for (int i = 0; i + 1 < V; ++i) key[i] = pop ? key[i + 1] : key[i];
       key[V - 1] = pop ? 0u : key[V - 1];
+    };
+    int n = 0;
+    for (; n < p.top_k; ++n) {
+      const uint32_t m = __reduce_max_sync(kFull, key[0] & ~kPos);
+      if (m <= kClosedKey) break;
+      take(n, m);
     }
     if (!exact) {
-      border = __reduce_max_sync(kFull, key[0] & ~kPos);   // what the last choice won against
+      uint32_t border = __reduce_max_sync(kFull, key[0] & ~kPos);   // what the last choice won against
       const uint32_t have = mine & ~kPos;
       uint32_t next = __shfl_down_sync(kFull, have, 1);
       if (lane == p.top_k - 1) next = border;
-      bool tie = have == next;
-      if (by_score) {
-        const float v = key_value(have), w = key_value(next);
-        tie = v - w <= 0x1p-16f * p_max + 0x1p-19f * (fabsf(v) + fabsf(w));
+      const float slack = 0x1p-16f * p_max;
+      auto tied = [&](uint32_t hi, uint32_t lo) {
+        const float v = key_value(hi), w = key_value(lo);
+        return by_score ? v - w <= slack + 0x1p-19f * (fabsf(v) + fabsf(w)) : hi == lo;
+      };
+      if (__any_sync(kFull, lane < p.top_k && have > kClosedKey && next > kClosedKey && tied(have, next))) {
+        // Everything that may belong to the top_k joins: what ties with the last choice.
+        const uint32_t last = __shfl_sync(kFull, have, p.top_k - 1);
+        while (n < 32 && border > kClosedKey && tied(last, border)) {
+          take(n++, border);
+          border = __reduce_max_sync(kFull, key[0] & ~kPos);
+        }
+        close = n == 32 && border > kClosedKey && tied(last, border);
+        if (!close) {
+          id = mine != 0 ? from * V + static_cast<int>(kPos - (mine & kPos)) : -1;
+          id = order_in_fp64<kBf16>(p, row, id, n, lane);
+          mine = 0;
+        }
       }
-      close = __any_sync(kFull, tie && lane < p.top_k && have > kClosedKey && next > kClosedKey);
     }
     if (mine != 0) id = from * V + static_cast<int>(kPos - (mine & kPos));
   }

@@ -8,13 +8,9 @@
 //
 // A slot that goes nowhere (id outside [0, experts)) has row -1 and is skipped everywhere; rows that no
 // slot names are never written.  No atomics: the order of every sum and of the rows is fixed.
-#include <cooperative_groups.h>
-
 #include "i8_common.cuh"
 #include "ptx.cuh"
 #include "quant_i8.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace smb {
 namespace {
@@ -52,100 +48,142 @@ struct DispatchParams {
 // One cluster sorts everything: warp w of the cluster owns the slots [w * per_warp, + per_warp), so
 // "earlier slots" means earlier lanes, earlier chunks, earlier warps, earlier CTAs, and the counts of the
 // CTAs meet through distributed shared memory instead of a second launch.
-//   shared: hist[warps][groups] | total[groups] | start[groups] | padded[groups]
+//   shared: hist[warps][groups] | total[groups] | start[groups] | count[groups]
+// Bound by latency: the ids of a warp are fetched together (8 x 32 at a time) and stay in registers
+// between the count and the placement where they fit.
+constexpr int kHeldIds = 8;
+
+__device__ __forceinline__ int clean_id(int e, int groups) { return e >= 0 && e < groups ? e : -1; }
+
+template <bool kCluster>
 __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) {
   extern __shared__ int sm[];
-  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ int warp_sums[32];
   griddep_launch_dependents();
-  griddep_wait();
   const int warps = blockDim.x >> 5;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int ctas = kCluster ? static_cast<int>(cluster_nctarank()) : 1;
+  const int rank = kCluster ? static_cast<int>(cluster_ctarank()) : 0;
   const int G = p.groups;
   int* hist = sm;
   int* total = hist + warps * G;
   int* start = total + G;
-  int* padded = start + G;
-  __shared__ int rows_used;
+  int* count = start + G;
 
-  for (int i = threadIdx.x; i < warps * G; i += blockDim.x) hist[i] = 0;
-  __syncthreads();
-  int* mine = hist + warp * G;
   const long long first = static_cast<long long>(rank * warps + warp) * p.per_warp;
   const int lo = static_cast<int>(first < p.n ? first : p.n);
   const int hi = static_cast<int>(first + p.per_warp < p.n ? first + p.per_warp : p.n);
-  for (int s0 = lo; s0 < hi; s0 += 32) {
-    const int s = s0 + lane;
-    int e = s < hi ? p.ids[s] : -1;
-    if (e < 0 || e >= G) e = -1;
-    const unsigned same = __match_any_sync(kFull, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  int* mine = hist + warp * G;
+  for (int e = lane; e < G; e += 32) mine[e] = 0;
+  griddep_wait();
+  int held[kHeldIds];
+#pragma unroll
+  for (int i = 0; i < kHeldIds; ++i) {
+    const int s = lo + i * 32 + lane;
+    held[i] = s < hi ? p.ids[s] : -1;
+  }
+  __syncwarp();
+  const bool fits = hi - lo <= kHeldIds * 32;
+  for (int s0 = lo; s0 < hi; s0 += kHeldIds * 32) {
+    if (s0 != lo) {
+#pragma unroll
+      for (int i = 0; i < kHeldIds; ++i) {
+        const int s = s0 + i * 32 + lane;
+        held[i] = s < hi ? p.ids[s] : -1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeldIds; ++i) {
+      if (s0 + i * 32 >= hi) break;
+      const int e = clean_id(held[i], G);
+      const unsigned same = __match_any_sync(kFull, e);
+      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
+  // Exclusive prefix of every group over the warps of this CTA.
   for (int e = threadIdx.x; e < G; e += blockDim.x) {
     int before = 0;
-    for (int w = 0; w < warps; ++w) {
-      const int c = hist[w * G + e];
-      hist[w * G + e] = before;
-      before += c;
+    for (int w0 = 0; w0 < warps; w0 += 8) {
+      int c[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c[i] = w0 + i < warps ? hist[(w0 + i) * G + e] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (w0 + i < warps) hist[(w0 + i) * G + e] = before;
+        before += c[i];
+      }
     }
     total[e] = before;
   }
-  cluster.sync();
-  for (int e = threadIdx.x; e < G; e += blockDim.x) {
+  if (kCluster) cluster_sync_all();   // also a CTA barrier
+  else __syncthreads();
+  // Threads take runs of groups; counts over all CTAs, then an exclusive scan of the padded sizes.
+  const int per = (G + blockDim.x - 1) / blockDim.x;   // 1 unless there are more groups than threads
+  const int e_lo = min(static_cast<int>(threadIdx.x) * per, G), e_hi = min(e_lo + per, G);
+  auto padded = [&](int c) { return p.align == 1 ? c : (c + p.align - 1) / p.align * p.align; };
+  int sum = 0;
+  for (int e = e_lo; e < e_hi; ++e) {
     int before = 0, all = 0;
-    for (int c = 0; c < ctas; ++c) {
-      const int v = *cluster.map_shared_rank(total + e, c);
-      if (c < rank) before += v;
-      all += v;
+    if (kCluster) {
+      const uint32_t addr = smem_u32(total + e);
+      int v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = c < ctas ? static_cast<int>(ld_shared_cluster_u32(mapa_u32(addr, c))) : 0;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c < rank) before += v[c];
+        all += v[c];
+      }
+    } else {
+      all = total[e];
     }
     start[e] = before;
-    padded[e] = all;
+    count[e] = all;
+    sum += padded(all);
   }
-  cluster.sync();   // also: nobody's shared memory is read by another CTA after this
-  if (warp == 0) {
-    // Exclusive scan of the padded counts: a run of groups per lane, then five shuffles.
-    const int per = (G + 31) / 32;
-    int sum = 0;
-    for (int i = 0; i < per; ++i) {
-      const int e = lane * per + i;
-      if (e < G) sum += (padded[e] + p.align - 1) / p.align * p.align;
-    }
-    int before = sum;
+  int inclusive = sum;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(kFull, before, d);
-      if (lane >= d) before += up;
-    }
-    if (lane == 31) rows_used = before;
-    before -= sum;
-    for (int i = 0; i < per; ++i) {
-      const int e = lane * per + i;
-      if (e < G) {
-        const int size = (padded[e] + p.align - 1) / p.align * p.align;
-        total[e] = before;                  // first row of the group, from here on
-        start[e] += before;
-        if (rank == 0) p.offsets[e] = before;
-        before += size;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int up = __shfl_up_sync(kFull, inclusive, d);
+    if (lane >= d) inclusive += up;
+  }
+  if (lane == 31) warp_sums[warp] = inclusive;
+  if (kCluster) cluster_sync_all();   // nobody's totals are read by another CTA after this
+  else __syncthreads();
+  const int others = lane < warps ? warp_sums[lane] : 0;
+  int base = __reduce_add_sync(kFull, lane < warp ? others : 0) + inclusive - sum;
+  const int used = __reduce_add_sync(kFull, others);
+  for (int e = e_lo; e < e_hi; ++e) {
+    total[e] = base;                  // first row of the group, from here on
+    start[e] += base;
+    if (rank == 0) p.offsets[e] = base;
+    base += padded(count[e]);
+  }
+  if (rank == 0 && threadIdx.x == 0) p.offsets[G] = used;
+  __syncthreads();
+  for (int s0 = lo; s0 < hi; s0 += kHeldIds * 32) {
+    if (!fits) {
+#pragma unroll
+      for (int i = 0; i < kHeldIds; ++i) {
+        const int s = s0 + i * 32 + lane;
+        held[i] = s < hi ? p.ids[s] : -1;
       }
     }
-    if (rank == 0 && lane == 31) p.offsets[G] = rows_used;
-  }
-  __syncthreads();
-  const int used = rows_used;
-  for (int s0 = lo; s0 < hi; s0 += 32) {
-    const int s = s0 + lane;
-    int e = s < hi ? p.ids[s] : -1;
-    if (e < 0 || e >= G) e = -1;
-    const unsigned same = __match_any_sync(kFull, e);
-    int row = -1;
-    if (e >= 0) row = start[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
-    __syncwarp();
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
-    if (s < hi) p.row_of_slot[s] = row;
-    if (row >= 0) p.slot_of_row[row] = s;
+#pragma unroll
+    for (int i = 0; i < kHeldIds; ++i) {
+      const int s = s0 + i * 32 + lane;
+      if (s0 + i * 32 >= hi) break;
+      const int e = clean_id(held[i], G);
+      const unsigned same = __match_any_sync(kFull, e);
+      const int row = e >= 0 ? start[e] + mine[e] + __popc(same & ((1u << lane) - 1u)) : -1;
+      __syncwarp();
+      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+      __syncwarp();
+      if (s < hi) p.row_of_slot[s] = row;
+      if (row >= 0) p.slot_of_row[row] = s;
+    }
   }
   // Rows that no slot names: the padding of every group, and everything behind the last one.
   const int threads = ctas * blockDim.x;
@@ -153,7 +191,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   if (p.align > 1) {
     for (int e = me >> 5; e < G; e += threads >> 5) {
       const int end = e + 1 < G ? total[e + 1] : used;
-      for (int r = total[e] + padded[e] + lane; r < end; r += 32) p.slot_of_row[r] = -1;
+      for (int r = total[e] + count[e] + lane; r < end; r += 32) p.slot_of_row[r] = -1;
     }
   }
   for (int r = used + me; r < p.cap; r += threads) p.slot_of_row[r] = -1;
@@ -200,12 +238,16 @@ __global__ void __launch_bounds__(kCta) gather_i8_kernel(const uint16_t* x, int6
                                                          int64_t tokens, int top_k, int width, int max_rows, int8_t* codes,
                                                          int64_t ld_bytes, float* scales) {
   __shared__ uint32_t red[kCta / 32];
+  __shared__ int rows_all[kCta / kThreads][kMaxTopKRows];
   griddep_launch_dependents();
   griddep_wait();
   const int tid = threadIdx.x % kThreads;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (kCta / kThreads) + threadIdx.x / kThreads;
   if (t >= tokens) return;   // whole warps, and whole CTAs where a row has more than one
-  const int* rows = row_of_slot + t * top_k;
+  // The destinations are fetched along with the row; quantize_row has a barrier between its loads and
+  // its stores.
+  int* rows = rows_all[threadIdx.x / kThreads];
+  if (tid < top_k) rows[tid] = row_of_slot[t * top_k + tid];
   const float scale = qi8::quantize_row<true, kThreads, 4, kAligned>(
       x + t * ld_x, width, tid, red,
       [&](int k, uint2 c) {
@@ -248,24 +290,41 @@ __global__ void __launch_bounds__(kCta) combine_kernel(const uint16_t* rows_in, 
   float acc[8] = {};
   const int n = min(8, width - c0);
   const bool whole = kAligned && n == 8;
-#pragma unroll 4
-  for (int j = 0; j < top_k; ++j) {
-    const int r = rows[j];
-    if (r < 0 || r >= max_rows) continue;
-    const float w = weights != nullptr ? weights[t * top_k + j] : 1.0f;
-    const uint16_t* src = rows_in + static_cast<int64_t>(r) * ld_rows + c0;
-    if (whole) {
-      const uint4 q = *reinterpret_cast<const uint4*>(src);
-      const uint32_t v[4] = {q.x, q.y, q.z, q.w};
+  const float* w_row = weights != nullptr ? weights + t * top_k : nullptr;
+  // Eight slots at a time: their rows, then all their loads, are in flight together.
+  for (int j0 = 0; j0 < top_k; j0 += 8) {
+    int r[8];
+    float w[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[2 * i] = fmaf(w, bf16_lo(v[i]), acc[2 * i]);
-        acc[2 * i + 1] = fmaf(w, bf16_hi(v[i]), acc[2 * i + 1]);
+    for (int i = 0; i < 8; ++i) {
+      r[i] = j0 + i < top_k ? rows[j0 + i] : -1;
+      w[i] = w_row != nullptr && j0 + i < top_k ? w_row[j0 + i] : 1.0f;
+      if (r[i] >= max_rows) r[i] = -1;
+    }
+    if (whole) {
+      uint4 q[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r[i] >= 0) q[i] = *reinterpret_cast<const uint4*>(rows_in + static_cast<int64_t>(r[i]) * ld_rows + c0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r[i] < 0) continue;
+        const uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          acc[2 * k] = fmaf(w[i], bf16_lo(v[k]), acc[2 * k]);
+          acc[2 * k + 1] = fmaf(w[i], bf16_hi(v[k]), acc[2 * k + 1]);
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) acc[i] = fmaf(w, bf16_one(src[i]), acc[i]);
+      for (int i = 0; i < 8; ++i) {
+        if (r[i] < 0) continue;
+        const uint16_t* src = rows_in + static_cast<int64_t>(r[i]) * ld_rows + c0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k < n) acc[k] = fmaf(w[i], bf16_one(src[k]), acc[k]);
+      }
     }
   }
   uint16_t* dst = y + t * ld_y + c0;
@@ -419,17 +478,20 @@ extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int t
   if (warps > 32) warps = 32;
   p.per_warp = static_cast<int>((p.n + static_cast<int64_t>(ctas) * warps * 32 - 1) / (static_cast<int64_t>(ctas) * warps * 32)) * 32;
   const size_t smem = static_cast<size_t>(warps + 3) * groups * sizeof(int);
-  cudaError_t e = cudaFuncSetAttribute(dispatch_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       35 * kMaxDispatchGroups * static_cast<int>(sizeof(int)));
-  if (e != cudaSuccess) return set_cuda_error(e, "dispatch shared memory");
+  auto kernel = ctas > 1 ? dispatch_kernel<true> : dispatch_kernel<false>;
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         35 * kMaxDispatchGroups * static_cast<int>(sizeof(int)));
+    if (e != cudaSuccess) return set_cuda_error(e, "dispatch shared memory");
+  }
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, 1, 1), dim3(warps * 32, 1, 1), smem, static_cast<cudaStream_t>(stream), attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.numAttrs = 2;
-  return finish(cudaLaunchKernelEx(&cfg, dispatch_kernel, p), "dispatch launch");
+  cfg.numAttrs = ctas > 1 ? 2 : 1;
+  return finish(cudaLaunchKernelEx(&cfg, kernel, p), "dispatch launch");
 }
 
 extern "C" int smb_moe_gather_bf16_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens,

@@ -103,7 +103,7 @@ __host__ __device__ inline RowScale row_scale(float amax, bool finite) {
 
 // One row by `kThreads` threads of a CTA (32: a warp, no barrier; more: `red` holds one word per warp
 // of the CTA, and the CTA's threads belong to one row).  `store8(k, codes)` and `store1(k, code)`
-// receive the codes; returns the row's scale.  kVecs vectors per thread stay in registers between the
+// receive the codes, after a barrier of the row's threads; returns the row's scale.  kVecs vectors per thread stay in registers between the
 // two passes, longer rows are read again (from L2).
 template <bool kBf16, int kThreads, int kVecs, bool kAligned, class Store8, class Store1>
 __device__ __forceinline__ float quantize_row(const void* row, int K, int tid, uint32_t* red, Store8 store8,
@@ -124,6 +124,7 @@ __device__ __forceinline__ float quantize_row(const void* row, int K, int tid, u
   for (int k = nvec * 8 + tid; k < K; k += kThreads)
     m = max(m, __float_as_uint(load_one<kBf16>(row, k)) & 0x7FFFFFFFu);
   m = __reduce_max_sync(0xffffffffu, m);
+  __syncwarp();   // what the caller put into shared memory is there for store8 / store1
   if (kThreads > 32) {
     if ((tid & 31) == 0) red[tid >> 5] = m;
     __syncthreads();
