@@ -57,7 +57,6 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kFull, k); }
 __device__ __forceinline__ unsigned long long warp_max(unsigned long long k) {
   const uint32_t hi = static_cast<uint32_t>(k >> 32);
   const uint32_t top = __reduce_max_sync(kFull, hi);
@@ -138,8 +137,10 @@ struct Top2 {
   }
 };
 
-// The whole choice on fp64 scores: for tokens whose groups, or more experts than a warp has lanes, lie
-// closer together than fp32 can tell.
+__device__ __forceinline__ float key_score(uint32_t k) { return k > kClosedKey ? key_value(k) : -INFINITY; }
+
+// The whole choice on fp64 scores: for tokens with more experts than a warp has lanes closer together
+// than fp32 can tell.
 // `s` holds experts doubles of this warp.  Returns lane j's choice j.
 template <bool kBf16>
 __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row, double* s, int lane) {
@@ -149,6 +150,7 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
   for (int e = lane; e < p.experts; e += 32) top = fmaxf(top, clean_logit(load_logit<kBf16>(row, e)));
   top = warp_max_float(top);
   double sum = 0.0;
+#pragma unroll 4
   for (int e = lane; e < p.experts; e += 32) {
     const float l = clean_logit(load_logit<kBf16>(row, e));
     double v = 0.0;
@@ -157,6 +159,7 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
     sum += v;
   }
   sum = sigmoid ? 1.0 : warp_sum(sum);
+#pragma unroll 4
   for (int e = lane; e < p.experts; e += 32) {
     const bool open = clean_logit(load_logit<kBf16>(row, e)) > -INFINITY;
     const double v = s[e] / sum + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
@@ -189,6 +192,7 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
   for (int j = 0; j < p.top_k; ++j) {
     unsigned long long best = 0;
     int at = 0;
+#pragma unroll 4
     for (int e = lane; e < p.experts; e += 32) {
       const unsigned long long k = s[e] > -INFINITY ? order_key(s[e]) : 0ull;
       if (k > best) {
@@ -204,6 +208,70 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
     __syncwarp();
   }
   return id;
+}
+
+// The open groups from fp64 scores.  The lane's V exponentials are independent of one another, which is
+// what keeps this short: a token in a thousand comes here and the last of them sets the kernel's end.
+template <int V, bool kBf16>
+__device__ __noinline__ uint32_t groups_in_fp64(const RouteParams& p, const void* row, double* buf, int lane) {
+  const bool sigmoid = (p.flags & SMB_ROUTE_SIGMOID) != 0;
+  const int e0 = lane * V;
+  float l[V], b[V];
+  load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
+#pragma unroll
+  for (int i = 0; i < V; ++i) b[i] = 0.0f;
+  if (p.bias != nullptr) load_run<V, false>(p.bias, e0, p.experts, p.bias_wide, b);
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    l[i] = clean_logit(l[i]);
+    top = fmaxf(top, l[i]);
+  }
+  top = fmaxf(warp_max_float(top), -FLT_MAX);
+  double s[V], sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const double e = exp(sigmoid ? -static_cast<double>(l[i]) : static_cast<double>(l[i]) - top);
+    s[i] = sigmoid ? 1.0 / (1.0 + e) : e;
+    sum += s[i];
+  }
+  if (!sigmoid) {
+    sum = warp_sum(sum);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = sum > 0.0 ? s[i] / sum : 0.0;
+  }
+  Top2<double> best = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    s[i] += b[i];
+    s[i] = l[i] > -INFINITY && s[i] > -INFINITY ? s[i] : -INFINITY;
+  }
+  const bool top2 = (p.flags & SMB_ROUTE_GROUP_TOP2) != 0;
+  double value;
+  if (p.group_lanes != 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) best.add(s[i]);
+    for (int d = 1; d < p.group_lanes; d <<= 1) {
+      const Top2<double> o = {__shfl_xor_sync(kFull, best.best, d), __shfl_xor_sync(kFull, best.second, d)};
+      best.join(o);
+    }
+    value = __shfl_sync(kFull, best.value(top2), lane * p.group_lanes);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (e0 + i < p.experts) buf[e0 + i] = s[i];
+    __syncwarp();
+    if (lane < p.n_groups)
+      for (int i = 0; i < p.group_size; ++i) best.add(buf[lane * p.group_size + i]);
+    __syncwarp();
+    value = best.value(top2);
+  }
+  int ahead = 0;
+  for (int g = 0; g < p.n_groups; ++g) {
+    const double other = __shfl_sync(kFull, value, g);
+    ahead += other > value || (other == value && g < lane) ? 1 : 0;
+  }
+  return __ballot_sync(kFull, lane < p.n_groups && ahead < p.top_groups);
 }
 
 // Lanes 0 .. n - 1 hold the ids of all experts that can be among the top_k; their fp64 scores (logits
@@ -274,8 +342,8 @@ __device__ __forceinline__ void sort_down(uint32_t (&k)[V]) {
 // winner's list.  The bits that the position covers are made good like the rounding of exp: neighbours
 // closer than their worth go to the fp64 choice.
 template <int V, bool kBf16>
-__global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(const RouteParams p) {
-  __shared__ double buf_all[kWarps][kMaxExperts];
+__global__ void __launch_bounds__(kWarps * 32, V <= 2 ? 16 : (V <= 8 ? 12 : 6)) route_kernel(const RouteParams p) {
+  __shared__ double buf_all[kWarps][V * 32];
   griddep_launch_dependents();
   griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -291,10 +359,10 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
   const int e0 = lane * V;   // lanes hold runs of V experts, so lower lanes hold lower indices
   float l[V];
   load_run<V, kBf16>(row, e0, p.experts, p.wide, l);
-#pragma unroll
-  for (int i = 0; i < V; ++i) l[i] = clean_logit(l[i]);
   float top = 0.0f;
   if (!sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] = clean_logit(l[i]);
     top = l[0];
 #pragma unroll
     for (int i = 1; i < V; ++i) top = fmaxf(top, l[i]);
@@ -302,13 +370,15 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
   }
 
   uint32_t key[V];
-  float p_max = 0.0f;
-  bool close = false;
+  float p_max = 0.0f, slack = 0.0f;
   if (by_score || by_group) {
     float s[V];
     constexpr float kLog2e = 1.4426950408889634f;
-    // exp as one product and ex2.approx: off by (2 + 1.2 |l|) steps of 2^-24 relative, which the
-    // thresholds below allow for (2^-16 of the largest p for two scores).
+    // exp as one product and ex2.approx is off by (2 + 1.2 |argument|) u relative, u = 2^-24.
+    // Sigmoid: that times (1 - p), and 1.5 u for the sum and the reciprocal; |l| p is largest at the
+    // largest p, where |l| < 0.7 (number of binary places of p + 1).  Softmax: at most 2.2 u of the largest
+    // p, and common factors (the sum over V values and five shuffles, its reciprocal) below 16 u.  So
+    // `slack` bounds the error of the difference of two scores.
     if (sigmoid) {
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] = rcp_approx(1.0f + ex2_approx(-l[i] * kLog2e));   // closed: 1 / (1 + inf) = 0
@@ -328,6 +398,8 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
 #pragma unroll
     for (int i = 0; i < V; ++i) p_max = fmaxf(p_max, s[i]);
     p_max = __uint_as_float(__reduce_max_sync(kFull, __float_as_uint(p_max)));   // p >= 0: bits order as they are
+    const int places = 127 - static_cast<int>(__float_as_uint(p_max) >> 23);
+    slack = 0x1p-23f * p_max * (sigmoid ? 6.0f + static_cast<float>(places) : 20.0f);
     if (by_score) {
       float b[V];
       load_run<V, false>(p.bias, e0, p.experts, p.bias_wide, b);
@@ -337,17 +409,23 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       s[i] = l[i] > -INFINITY ? fmaxf(s[i], -INFINITY) : -INFINITY;   // a bias of -inf or NaN closes an expert too
-      key[i] = (order_key(by_score ? s[i] : l[i]) & ~kPos) | (kPos - i);
+      key[i] = (order_key(by_score ? s[i] : fmaxf(l[i], -INFINITY)) & ~kPos) | (kPos - i);
     }
+    sort_down<V>(key);
     if (by_group) {
       Top2<float> best = {-INFINITY, -INFINITY};
       const bool top2 = (p.flags & SMB_ROUTE_GROUP_TOP2) != 0;
       float value = -INFINITY;   // lane g: value of group g
       const int lanes = p.group_lanes;
       if (lanes != 0) {
-        // A group is a run of 2^n whole lanes: join them by shuffles.
+        // A group is a run of 2^n whole lanes: join them by shuffles.  Keys of scores are sorted already.
+        if (by_score) {
+          best.best = key_score(key[0] & ~kPos);
+          if (V > 1) best.second = key_score(key[V > 1 ? 1 : 0] & ~kPos);
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) best.add(s[i]);
+          for (int i = 0; i < V; ++i) best.add(s[i]);
+        }
         for (int d = 1; d < lanes; d <<= 1) {
           const Top2<float> o = {__shfl_xor_sync(kFull, best.best, d), __shfl_xor_sync(kFull, best.second, d)};
           best.join(o);
@@ -372,48 +450,42 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
         ahead += other > gkey || (other == gkey && g < lane) ? 1 : 0;
       }
       const bool in = lane < p.n_groups && ahead < p.top_groups;
-      const uint32_t kept = __ballot_sync(kFull, in);
+      uint32_t kept = __ballot_sync(kFull, in);
       // Only the border matters: the last group kept against the first left out.
       const uint32_t last = __reduce_min_sync(kFull, in ? gkey : 0xFFFFFFFFu);
       const uint32_t first = __reduce_max_sync(kFull, in ? 0u : gkey);
       if (first > kClosedKey) {
         const float v = key_value(last), w = key_value(first);
-        close = v - w <= 0x1p-15f * p_max + 0x1p-21f * (fabsf(v) + fabsf(w));
+        // Sums of up to two scores, each with its rounding and hidden position bits.
+        if (v - w <= 2.0f * slack + 0x1p-23f * (kPos + 3) * (fabsf(v) + fabsf(w)))
+          kept = groups_in_fp64<V, kBf16>(p, row, buf_all[warp], lane);
       }
       if (lanes != 0) {
-        const bool closed = !((kept >> ((lane >> (31 - __clz(lanes))) & 31)) & 1u);
-#pragma unroll
-        for (int i = 0; i < V; ++i) key[i] = closed ? 0u : key[i];
+        // A closed lane never wins, so its head alone keeps it out.
+        if (!((kept >> ((lane >> (31 - __clz(lanes))) & 31)) & 1u)) key[0] = 0;
       } else {
-        int g = e0 / p.group_size, in_group = e0 - g * p.group_size;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+          const int g = (e0 + static_cast<int>(kPos - (key[i] & kPos))) / p.group_size;
           key[i] = ((kept >> (g & 31)) & 1u) ? key[i] : 0u;
-          if (++in_group == p.group_size) {
-            in_group = 0;
-            ++g;
-          }
         }
+        sort_down<V>(key);
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = (order_key(l[i]) & ~kPos) | (kPos - i);
+    for (int i = 0; i < V; ++i) key[i] = (order_key(fmaxf(l[i], -INFINITY)) & ~kPos) | (kPos - i);
+    sort_down<V>(key);
   }
 
   int id = -1;
-  if (!close) {
-    sort_down<V>(key);
-    uint32_t mine = 0;   // lane j: key and lane of the j-th best
-    int from = 0;
+  bool close = false;
+  {
+    uint2* won = reinterpret_cast<uint2*>(buf_all[warp]);   // key and lane of the j-th best
     auto take = [&](int j, uint32_t m) {
       const int win = __ffs(__ballot_sync(kFull, (key[0] & ~kPos) == m)) - 1;   // lanes hold ascending experts
-      const uint32_t k = __shfl_sync(kFull, key[0], win);
-      if (lane == j) {
-        mine = k;
-        from = win;
-      }
       const bool pop = lane == win;
+      if (pop) won[j] = make_uint2(key[0], lane);
 #pragma unroll
       for (int i = 0; i + 1 < V; ++i) key[i] = pop ? key[i + 1] : key[i];
       key[V - 1] = pop ? 0u : key[V - 1];
@@ -424,15 +496,17 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
       if (m <= kClosedKey) break;
       take(n, m);
     }
+    __syncwarp();
+    uint32_t mine = lane < n ? won[lane].x : 0u;   // lane j: the j-th best
     if (!exact) {
       uint32_t border = __reduce_max_sync(kFull, key[0] & ~kPos);   // what the last choice won against
       const uint32_t have = mine & ~kPos;
       uint32_t next = __shfl_down_sync(kFull, have, 1);
       if (lane == p.top_k - 1) next = border;
-      const float slack = 0x1p-16f * p_max;
       auto tied = [&](uint32_t hi, uint32_t lo) {
         const float v = key_value(hi), w = key_value(lo);
-        return by_score ? v - w <= slack + 0x1p-19f * (fabsf(v) + fabsf(w)) : hi == lo;
+        // The rounding of p + bias, and the steps that the position bits hide.
+        return by_score ? v - w <= slack + 0x1p-23f * (kPos + 2) * (fabsf(v) + fabsf(w)) : hi == lo;
       };
       if (__any_sync(kFull, lane < p.top_k && have > kClosedKey && next > kClosedKey && tied(have, next))) {
         // Everything that may belong to the top_k joins: what ties with the last choice.
@@ -441,15 +515,18 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
           take(n++, border);
           border = __reduce_max_sync(kFull, key[0] & ~kPos);
         }
+        __syncwarp();
+        mine = lane < n ? won[lane].x : 0u;
         close = n == 32 && border > kClosedKey && tied(last, border);
         if (!close) {
-          id = mine != 0 ? from * V + static_cast<int>(kPos - (mine & kPos)) : -1;
+          id = mine != 0 ? static_cast<int>(won[lane].y * V + kPos - (mine & kPos)) : -1;
           id = order_in_fp64<kBf16>(p, row, id, n, lane);
           mine = 0;
         }
       }
     }
-    if (mine != 0) id = from * V + static_cast<int>(kPos - (mine & kPos));
+    if (mine != 0) id = static_cast<int>(won[lane].y * V + kPos - (mine & kPos));
+    __syncwarp();
   }
   if (close) id = choose_in_fp64<kBf16>(p, row, buf_all[warp], lane);
 

@@ -17,14 +17,24 @@ from . import capi
 from .gemm import _ptr, _stream_ptr
 
 
+def _addr(x):
+    """Address of a device buffer; the common kinds first, since a decode step makes many of these calls."""
+    if x is None:
+        return None
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
+
+
 def route_device(logits, ids, weights, tokens: int, experts: int, top_k: int, dtype: int = capi.DTYPE_F32, bias=None,
                  n_groups: int = 1, top_groups: int = 1, flags: int = 0, scale: float = 1.0, ld: int | None = None,
                  stream=None) -> None:
     """ids [tokens, top_k] int32 and weights [tokens, top_k] fp32 from logits [tokens, experts]; closed
     slots hold id -1, weight 0.  `flags`: capi.ROUTE_*."""
     capi.check(capi.lib().smb_moe_route_device(
-        _ptr(logits), dtype, experts if ld is None else ld, _ptr(bias), tokens, experts, top_k, n_groups, top_groups,
-        flags, scale, _ptr(ids), _ptr(weights), _stream_ptr(stream)))
+        _addr(logits), dtype, experts if ld is None else ld, _addr(bias), tokens, experts, top_k, n_groups, top_groups,
+        flags, scale, _addr(ids), _addr(weights), _stream_ptr(stream)))
 
 
 def route_backward_device(logits, ids, grad_weights, grad_logits, tokens: int, experts: int, top_k: int,
@@ -32,8 +42,8 @@ def route_backward_device(logits, ids, grad_weights, grad_logits, tokens: int, e
                           ld_grad: int | None = None, stream=None) -> None:
     """grad_logits [tokens, experts] for the ids of the forward pass."""
     capi.check(capi.lib().smb_moe_route_backward_device(
-        _ptr(logits), dtype, experts if ld is None else ld, _ptr(ids), _ptr(grad_weights), tokens, experts, top_k, flags,
-        scale, _ptr(grad_logits), experts if ld_grad is None else ld_grad, _stream_ptr(stream)))
+        _addr(logits), dtype, experts if ld is None else ld, _addr(ids), _addr(grad_weights), tokens, experts, top_k, flags,
+        scale, _addr(grad_logits), experts if ld_grad is None else ld_grad, _stream_ptr(stream)))
 
 
 def max_rows(tokens: int, top_k: int, groups: int, align: int = 1) -> int:
@@ -46,15 +56,15 @@ def dispatch_device(ids, offsets, row_of_slot, slot_of_row, tokens: int, top_k: 
     """Stable sort of the slots by expert: offsets [groups + 1], row_of_slot [tokens, top_k], slot_of_row
     [max_rows], and with align = 256 the tile map of Bf16Plan.grouped."""
     capi.check(capi.lib().smb_moe_dispatch_device(
-        _ptr(ids), tokens, top_k, groups, align, max_rows, _ptr(offsets), _ptr(row_of_slot), _ptr(slot_of_row),
-        _ptr(mtile_group), _stream_ptr(stream)))
+        _addr(ids), tokens, top_k, groups, align, max_rows, _addr(offsets), _addr(row_of_slot), _addr(slot_of_row),
+        _addr(mtile_group), _stream_ptr(stream)))
 
 
 def gather_bf16_device(x, row_of_slot, out, tokens: int, top_k: int, width: int, max_rows: int, ld_x: int | None = None,
                        ld_out: int | None = None, stream=None) -> None:
     """Row row_of_slot[t, j] of `out` [max_rows, width] becomes row t of x."""
     capi.check(capi.lib().smb_moe_gather_bf16_device(
-        _ptr(x), width if ld_x is None else ld_x, _ptr(row_of_slot), tokens, top_k, width, max_rows, _ptr(out),
+        _addr(x), width if ld_x is None else ld_x, _addr(row_of_slot), tokens, top_k, width, max_rows, _addr(out),
         width if ld_out is None else ld_out, _stream_ptr(stream)))
 
 
@@ -62,16 +72,16 @@ def gather_i8_device(x, row_of_slot, codes, scales, tokens: int, top_k: int, wid
                      ld_x: int | None = None, ld_bytes: int | None = None, stream=None) -> None:
     """The same with the rows quantised: int8 codes [max_rows, width] and scales [max_rows]."""
     capi.check(capi.lib().smb_moe_gather_i8_device(
-        _ptr(x), width if ld_x is None else ld_x, _ptr(row_of_slot), tokens, top_k, width, max_rows, _ptr(codes),
-        width if ld_bytes is None else ld_bytes, _ptr(scales), _stream_ptr(stream)))
+        _addr(x), width if ld_x is None else ld_x, _addr(row_of_slot), tokens, top_k, width, max_rows, _addr(codes),
+        width if ld_bytes is None else ld_bytes, _addr(scales), _stream_ptr(stream)))
 
 
 def combine_device(rows, row_of_slot, weights, y, tokens: int, top_k: int, width: int, max_rows: int,
                    ld_rows: int | None = None, ld_y: int | None = None, stream=None) -> None:
     """y[t] = sum_j weights[t, j] * rows[row_of_slot[t, j]]; weights None: plain sum (the gradient of a gather)."""
     capi.check(capi.lib().smb_moe_combine_device(
-        _ptr(rows), width if ld_rows is None else ld_rows, _ptr(row_of_slot), _ptr(weights), tokens, top_k, width, max_rows,
-        _ptr(y), width if ld_y is None else ld_y, _stream_ptr(stream)))
+        _addr(rows), width if ld_rows is None else ld_rows, _addr(row_of_slot), _addr(weights), tokens, top_k, width, max_rows,
+        _addr(y), width if ld_y is None else ld_y, _stream_ptr(stream)))
 
 
 def combine_backward_device(grad_y, rows, row_of_slot, weights, grad_rows, grad_weights, tokens: int, top_k: int,
@@ -79,6 +89,6 @@ def combine_backward_device(grad_y, rows, row_of_slot, weights, grad_rows, grad_
                             ld_grad_rows: int | None = None, stream=None) -> None:
     """Gradients of combine_device: of the rows (those that a slot names) and, unless None, of the weights."""
     capi.check(capi.lib().smb_moe_combine_backward_device(
-        _ptr(grad_y), width if ld_grad_y is None else ld_grad_y, _ptr(rows), width if ld_rows is None else ld_rows,
-        _ptr(row_of_slot), _ptr(weights), tokens, top_k, width, max_rows, _ptr(grad_rows),
-        width if ld_grad_rows is None else ld_grad_rows, _ptr(grad_weights), _stream_ptr(stream)))
+        _addr(grad_y), width if ld_grad_y is None else ld_grad_y, _addr(rows), width if ld_rows is None else ld_rows,
+        _addr(row_of_slot), _addr(weights), tokens, top_k, width, max_rows, _addr(grad_rows),
+        width if ld_grad_rows is None else ld_grad_rows, _addr(grad_weights), _stream_ptr(stream)))
