@@ -314,7 +314,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
                              static_cast<uint32_t>((NB == 1) ? bank * TN + tile_col : tile_col);
       constexpr int kOutCols = kSwiglu ? C::kColsPerWarp / 2 : C::kColsPerWarp;
       uint32_t packed[kOutCols / 2];
-      drain_columns_i8<C::kColsPerWarp, kSwiglu>(taddr, sbuf, sa, packed);
+      drain_columns_i8<C::kColsPerWarp, kSwiglu, NB == 1>(taddr, sbuf, sa, packed);
       release_columns(leader_acc_empty0 + 8u * slot, lane);
       store_columns<kOutCols, kTmaStore>(packed, sbuf, out, row0, kSwiglu ? col0 / 2 : col0, lane);
     }
