@@ -45,6 +45,10 @@ constexpr int kWBytes = 128 * kBlockKBytes;   // 16 KiB weight box
 constexpr int kSfBytes = 1024;        // one 128-row band x 8 scales (two 512-byte cells)
 constexpr int kSlotCols = 16;         // SFW cells (8 columns) + SFX cells (8 columns) per stage
 constexpr int kMaxStages = 16;
+// These kernels take all 512 columns of tensor memory after they have let the next kernel start.  More than
+// half of an SM's shared memory, however few stages are asked for, keeps that kernel's tensor memory (which it
+// may hold while it waits for this one) off their SMs.
+constexpr int kMinSmem = 118 * 1024;
 constexpr int kDefaultStages = 6;
 constexpr int kDualFromPad = 16;      // padded activation rows from which two tiles share one activation box
 constexpr int kWholeTileStages = 8;
@@ -1290,7 +1294,8 @@ int fp4_decode_dual_launch(const Fp4DecodeLaunch& L, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(kFused ? fp4d::kFusedThreads : fp4d::kDualThreads, 1, 1);
-  cfg.dynamicSmemBytes = 1024 + stages * p.stage_bytes + staging + fp4d::kBarrierBytes;
+  const int smem = 1024 + stages * p.stage_bytes + staging + fp4d::kBarrierBytes;
+  cfg.dynamicSmemBytes = smem > fp4d::kMinSmem ? smem : fp4d::kMinSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1421,7 +1426,7 @@ int fp4_decode_launch(const Fp4DecodeLaunch& L, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, 1, 1);
   cfg.blockDim = dim3(fp4d::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = smem > fp4d::kMinSmem ? smem : fp4d::kMinSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
