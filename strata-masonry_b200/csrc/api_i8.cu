@@ -96,7 +96,8 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
   L.groups = g.groups;
   L.offsets = g.offsets;
   L.weights_static = (g.flags & SMB_FLAG_WEIGHTS_STATIC) != 0;
-  i8_pick_tile(g.M, g.N, g.K, device_cluster_slots(), &L.tile_n, &L.sub_blocks);
+  // Groups end inside a row tile: half a tile each on average.
+  i8_pick_tile(g.offsets != nullptr ? g.M + g.groups * 128 : g.M, g.N, g.K, device_cluster_slots(), &L.tile_n, &L.sub_blocks);
   if (g.flags & SMB_FLAG_TILE_N_512) { L.tile_n = 256; L.sub_blocks = 2; }
   if (g.flags & SMB_FLAG_TILE_N_256) { L.tile_n = 256; L.sub_blocks = 1; }
   if (g.flags & SMB_FLAG_TILE_N_128) { L.tile_n = 128; L.sub_blocks = 1; }
@@ -110,13 +111,18 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
   const bool tiled_only = (g.flags & (SMB_FLAG_NO_DECODE | SMB_FLAG_TILE_N_128 | SMB_FLAG_TILE_N_256 | SMB_FLAG_TILE_N_512)) != 0;
   L.decode = !tiled_only && i8_pick_decode(g.M, g.N, g.K, g.offsets != nullptr ? (g.groups < 2 ? 2 : g.groups) : 1,
                                            (g.flags & SMB_FLAG_DECODE_SINGLE) != 0, &L.chunk, &L.box_rows);
+  if (act_src != nullptr && i8_decode_fuses(L, act_src, act_ld)) {
+    L.x = static_cast<const uint16_t*>(act_src);
+    L.ldx = act_ld;
+  }
+  const bool own_codes = act_src != nullptr && L.x == nullptr;
   const void* a = g.a;
   int64_t lda = g.lda;
   L.sa = g.sa;
   if (rc == SMB_OK) {
     cudaError_t e = cudaMalloc(&p->status_dev, sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(p->status_dev, 0, sizeof(int));
-    if (act_src != nullptr) {
+    if (own_codes) {
       p->act_pitch = (static_cast<int64_t>(g.K) + 15) / 16 * 16;
       if (e == cudaSuccess) e = cudaMalloc(&p->act_codes, static_cast<size_t>(g.M) * p->act_pitch);
       if (e == cudaSuccess) e = cudaMalloc(&p->act_scales, static_cast<size_t>(g.M) * sizeof(float));
@@ -126,7 +132,8 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
     }
     if (e != cudaSuccess) rc = set_cuda_error(e, "i8 plan: allocation");
   }
-  if (rc == SMB_OK) rc = encode_tmap_2d(&L.tmap_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, L.decode ? L.box_rows : 128, 128,
+  if (rc == SMB_OK && L.x == nullptr)
+    rc = encode_tmap_2d(&L.tmap_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, L.decode ? L.box_rows : 128, 128,
                         true);
   if (rc == SMB_OK)
     rc = encode_tmap_2d(&L.tmap_b, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, static_cast<uint64_t>(g.groups) * g.N, g.K, g.ldb,
@@ -191,7 +198,7 @@ extern "C" int smb_i8_plan_run(smb_i8_plan* plan, void* stream) {
   if (cudaGetDevice(&device) != cudaSuccess || device != plan->device)
     return set_error(SMB_ERR_INVALID, "i8 plan: created on device %d, run with device %d current", plan->device, device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (plan->act_src != nullptr) {
+  if (plan->act_src != nullptr && plan->launch.x == nullptr) {
     const I8Launch& L = plan->launch;
     int rc = quantize_i8_launch(plan->act_src, true, plan->act_ld, plan->act_codes, plan->act_pitch, plan->act_scales, L.M,
                                 L.K, st);
@@ -219,7 +226,8 @@ extern "C" int smb_i8_plan_describe(smb_i8_plan* plan, char* out, size_t capacit
   const I8Launch& L = plan->launch;
   if (L.decode) {
     snprintf(out, capacity, "i8 decode chunk=%d%s%s%s", L.chunk, L.swiglu ? " swiglu" : "",
-             L.offsets != nullptr ? " grouped" : "", plan->act_src != nullptr ? " bf16-activations" : "");
+             L.offsets != nullptr ? " grouped" : "",
+             plan->act_src == nullptr ? "" : (L.x != nullptr ? " bf16-activations fused" : " bf16-activations"));
     return SMB_OK;
   }
   snprintf(out, capacity, "i8 tile 256x%d store=%s%s%s", L.tile_n * L.sub_blocks,

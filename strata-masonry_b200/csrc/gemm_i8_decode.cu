@@ -9,10 +9,15 @@
 // warps 2-9 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs cuts the K loop of a
 // pair and adds its int32 partial sums through distributed shared memory: the sums are exact, so their
 // order does not matter, and there is neither workspace nor atomic.
+//
+// Up to 4 bf16 tokens are quantised in the kernel itself: every CTA finds the scales of all rows (4 x K
+// bf16 come from L2) and writes the codes of its own K range where the MMA reads them.
+// That saves a launch and a trip of the codes through L2 in front of the first MMA.
 #include "gemm_common.cuh"
 #include "i8_common.cuh"
 #include "i8_epilogue.cuh"
 #include "ptx.cuh"
+#include "quant_i8.cuh"
 
 namespace smb {
 
@@ -24,11 +29,20 @@ constexpr int kThreads = 320;
 constexpr int kMaxSplit = 8;
 constexpr int kWBytes = kTileRows * kBlockK;
 constexpr int kMaxStages = 12;
-constexpr int kBarBytes = 256;
+constexpr int kBarBytes = 384;
+constexpr int kFusedTokens = 4;       // most tokens quantised in the kernel
+constexpr int kFusedRows = 8;         // rows of their codes in shared memory: the smallest N of the MMA
+// K blocks of codes (1 KB each) beside the ring, which keeps five stages.  us with the quantiser inside / as
+// a launch of its own, 1, 4 and 8 tokens: 4096 x 4096 (8 blocks per CTA) 7.1 / 8.3, 7.6 / 8.4, 8.5 / 8.4;
+// 28672 x 8192 (64 blocks, two stages left) 44.6 / 39.9.
+constexpr int kFusedMaxBlocks = 24;
 constexpr int kTableBytes = (kI8MaxGroups + 8) * 4;
-// The whole of shared memory, whatever the ring needs: no other kernel that allocates tensor memory can
-// then share the SM, so no allocation ever waits for a CTA that waits for this kernel to end.
-constexpr int kTotal = 232448;
+// Half of an SM's shared memory, and at most half of its tensor memory: two CTAs share an SM, so the next
+// launch on the stream starts its prologue (and the loads of weights nobody writes) while this one drains.
+// Never less, so that there are never three, and an allocation of tensor memory always succeeds at once: a
+// CTA that holds some may be waiting for the very kernel that asks for more.  (Of the other kernels that
+// allocate it, the narrow BF16 and FP4 tiles take half an SM of both; the rest leave no room beside them.)
+constexpr int kTotal = 111 * 1024;
 constexpr int kRingBudget = kTotal - 1024 - kBarBytes - kTableBytes;
 
 struct Params {
@@ -47,6 +61,8 @@ struct Params {
   int groups;
   int* status;
   int weights_static;
+  const uint16_t* x;  // fused quantiser: bf16 tokens [M, K], 16-byte rows, and their pitch
+  long long ldx;
 };
 
 struct Tile {
@@ -119,8 +135,67 @@ __device__ __forceinline__ Tile find_tile(const Params& p, const int* table, int
   return r;
 }
 
-__device__ __forceinline__ float token_scale(const Params& p, const Tile& tile, int c) {
-  return c < tile.rows ? p.sa[tile.row0 + c] : 0.0f;
+__device__ __forceinline__ float token_scale(const float* sa, const Tile& tile, int c) {
+  return c < tile.rows ? sa[tile.row0 + c] : 0.0f;
+}
+
+// The eight epilogue warps quantise the tokens, 8 / (M rounded up to a power of two) warps a row: the
+// scale of every row to `sa`, the codes of K blocks [kb0, kb1) to x_base ([block][8 rows][128 bytes],
+// 128-byte swizzle).  The loads for the codes go out together with the first loads for the maximum and
+// wait in registers (up to kHeld per thread; the rest is read again).  `red`: eight words.
+__device__ __forceinline__ void quantize_tokens(const Params& p, int kb0, int kb1, uint32_t x_base, uint32_t sa, uint32_t red,
+                                                int warp, int lane) {
+  const int share = p.M <= 1 ? 8 : (p.M <= 2 ? 4 : 2);   // warps per row
+  const int r = warp / share;
+  const int threads = share * 32, tid = (warp % share) * 32 + lane;
+  const bool live = r < p.M;
+  const uint16_t* row = p.x + r * p.ldx;
+  constexpr int kBlockVecs = kBlockK / 8;
+  const int nvec = live ? p.K / 8 : 0;
+  const int first = kb0 * kBlockVecs + tid, end = min(nvec, kb1 * kBlockVecs);
+  constexpr int kHeld = 4, kBatch = 8;
+  qi8::Vec<true> held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (first + threads * i < end) held[i] = qi8::load_vec<true>(row, static_cast<int64_t>(first + threads * i) * 8);
+  uint32_t m = 0;
+  for (int v0 = tid; v0 < nvec; v0 += threads * kBatch) {
+    qi8::Vec<true> q[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (v0 + threads * i < nvec) q[i] = qi8::load_vec<true>(row, static_cast<int64_t>(v0 + threads * i) * 8);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i)
+      if (v0 + threads * i < nvec) m = qi8::abs_max_bits<true>(q[i], m);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(red + 4u * warp), "r"(m) : "memory");
+  asm volatile("bar.sync 1, 256;" ::: "memory");   // the eight epilogue warps
+  uint32_t other;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(other) : "r"(red + 4u * (r * share + lane % share)) : "memory");
+  m = __reduce_max_sync(0xffffffffu, other);
+  if (!live) return;
+  const qi8::RowScale rs = qi8::row_scale(__uint_as_float(m), m < 0x7F800000u);
+  auto store = [&](int v, const qi8::Vec<true>& q) {
+    const uint2 c = rs.bad ? make_uint2(0, 0) : qi8::encode<true>(q, rs.inv);
+    const int in_block = v % kBlockVecs;
+    const uint32_t dst = x_base + (v / kBlockVecs - kb0) * (kFusedRows * kBlockK) + r * kBlockK +
+                         (((in_block >> 1) ^ (r & 7)) << 4) + (in_block & 1) * 8;
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst), "r"(c.x), "r"(c.y) : "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+    if (first + threads * i < end) store(first + threads * i, held[i]);
+  for (int v0 = first + threads * kHeld; v0 < end; v0 += threads * kHeld) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (v0 + threads * i < end) held[i] = qi8::load_vec<true>(row, static_cast<int64_t>(v0 + threads * i) * 8);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (v0 + threads * i < end) store(v0 + threads * i, held[i]);
+  }
+  if (tid == 0)
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(sa + 4u * r), "f"(rs.bad ? __uint_as_float(0x7FC00000u) : rs.scale) : "memory");
 }
 
 // Two tokens (rows m, m + 1 of D) of this lane's channel n, already scaled.  Neighbouring lanes trade
@@ -151,8 +226,9 @@ __device__ __forceinline__ void store_pair(const Params& p, long long m, int val
 }
 
 // kSplit: the CTAs of a cluster share the K loop of ONE tile (the grid has a cluster for every tile).
-template <bool kSwiglu, bool kPairs, bool kSplit>
-__global__ void __launch_bounds__(kThreads, 1)
+// kFused: bf16 tokens (at most 4, a plain product), codes and scales made here.
+template <bool kSwiglu, bool kPairs, bool kSplit, bool kFused>
+__global__ void __launch_bounds__(kThreads, 2)
 gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
                       const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -165,6 +241,11 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
   auto acc_full_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStages + b); };
   auto acc_empty_bar = [&](int b) { return bar_base + 8u * (2 * kMaxStages + 2 + b); };
   const uint32_t tmem_slot = bar_base + 8u * (2 * kMaxStages + 4);
+  const uint32_t x_bar = bar_base + 8u * (2 * kMaxStages + 5);
+  const float* sa_smem = reinterpret_cast<const float*>(smem_raw + (bar_base + 320u - smem_u32(smem_raw)));
+  const uint32_t x_base = ring_base + p.stages * p.stage_bytes;   // kFused: codes of this CTA's K range
+  const float* scales = kFused ? sa_smem : p.sa;
+  constexpr int kWOnly = kFused ? 1 : 0;   // stages hold weights alone
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -185,11 +266,12 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       mbar_init(acc_full_bar(b), 1);
       mbar_init(acc_empty_bar(b), 8);
     }
+    if (kFused) mbar_init(x_bar, 8);
     fence_mbar_init_cluster();
   }
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmap_w);
-    tma_prefetch_desc(&tmap_x);
+    if (!kFused) tma_prefetch_desc(&tmap_x);
   }
   if (warp == 1) {
     tmem_alloc<1>(tmem_slot, p.tmem_cols);
@@ -210,7 +292,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     if (warp == 0) {
       const int nt = unit / ((p.M + p.chunk - 1) / p.chunk);
       const int rows = min(p.chunk, p.M);   // every chunk is loaded as whole boxes
-      const uint32_t bytes = kWBytes + ((rows + p.box_rows - 1) / p.box_rows) * p.box_rows * kBlockK;
+      const uint32_t bytes = kWBytes + (kWOnly ? 0 : ((rows + p.box_rows - 1) / p.box_rows) * p.box_rows * kBlockK);
       for (int s = 0; s < early; ++s) {
         if (elect_one()) {
           mbar_arrive_expect_tx(full_bar(s), bytes);
@@ -240,7 +322,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     bool ok = true;
     for (int t = unit; t < num_tiles && ok; t += units) {
       const Tile tile = find_tile(p, table, t, lane);
-      const int boxes = (tile.rows + p.box_rows - 1) / p.box_rows;
+      const int boxes = kWOnly ? 0 : (tile.rows + p.box_rows - 1) / p.box_rows;
       const uint32_t bytes = kWBytes + boxes * p.box_rows * kBlockK;
       const int row_w = tile.group * p.N + tile.col0;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -273,6 +355,10 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     uint32_t ph = 0;
     int local = 0;
     bool ok = true;
+    if (kFused && !mbar_wait(x_bar, 0)) {
+      report_status(p.status, kDevTimeoutActivations);
+      ok = false;
+    }
     for (int t = unit; t < num_tiles && ok; t += units, ++local) {
       const Tile tile = find_tile(p, table, t, lane);
       const int boxes = (tile.rows + p.box_rows - 1) / p.box_rows;
@@ -293,7 +379,8 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         tc_fence_after_sync();
         const uint32_t w_addr = ring_base + s * p.stage_bytes;
         const uint64_t desc_w = make_smem_desc(w_addr, 1024, 16, kSwizzle128B);
-        const uint64_t desc_x = make_smem_desc(w_addr + kWBytes, 1024, 16, kSwizzle128B);
+        const uint64_t desc_x = make_smem_desc(kFused ? x_base + (kb - kb0) * (kFusedRows * kBlockK) : w_addr + kWBytes, 1024, 16,
+                                               kSwizzle128B);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < kBlockK / 32; ++k)
@@ -312,13 +399,20 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int quarter = warp & 3;
     const int half = (warp - 2) >> 2;
     int local = 0;
+    if (kFused) {
+      quantize_tokens(p, kb0, kb1, x_base, bar_base + 320u, bar_base + 352u, warp - 2, lane);
+      fence_proxy_async_smem();   // the MMA reads the codes through the async proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x_bar);
+      if (!mbar_wait(x_bar, 0) && lane == 0) report_status(p.status, kDevTimeoutActivations);   // all scales are there
+    }
     for (int t = unit; t < num_tiles; t += units, ++local) {
       const Tile tile = find_tile(p, table, t, lane);
       const int bank = local & 1;
       const int n = tile.col0 + quarter * 32 + lane;
       const float sb = !kSplit && n < p.N ? p.sb[static_cast<long long>(tile.group) * p.N + n] : 0.0f;
       // Lane i holds the scale of token i of the warp's current 16.
-      float sa = !kSplit ? token_scale(p, tile, half * 16 + (lane & 15)) : 0.0f;
+      float sa = !kSplit ? token_scale(scales, tile, half * 16 + (lane & 15)) : 0.0f;
       if (!mbar_wait(acc_full_bar(bank), static_cast<uint32_t>(local >> 1) & 1u)) {
         if (lane == 0) report_status(p.status, kDevTimeoutEpilogue);
         break;
@@ -337,7 +431,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
                          : "memory");
         } else {
           const float scale = sa;
-          sa = token_scale(p, tile, c0 + 32 + (lane & 15));
+          sa = token_scale(scales, tile, c0 + 32 + (lane & 15));
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
             const int c = c0 + i;
@@ -367,7 +461,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     cluster_sync_all();
     if (warp >= 2) {
       for (int c = rank * per + ((warp - 2) >> 2) * 4; c < end; c += 8) {
-        const float sa = token_scale(p, tile, c + (lane & 3));
+        const float sa = token_scale(scales, tile, c + (lane & 3));
         const uint32_t addr = ring_base + (c * kTileRows + quarter * 32 + lane) * 4;
         uint32_t part[kMaxSplit][4];
 #pragma unroll
@@ -403,9 +497,9 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
 namespace {
 
-template <bool kSwiglu, bool kPairs, bool kSplit>
+template <bool kSwiglu, bool kPairs, bool kSplit, bool kFused>
 int launch_i8_decode(const I8Launch& L, const i8d::Params& p, int ctas, int split, cudaStream_t stream) {
-  auto kernel = i8d::gemm_i8_decode_kernel<kSwiglu, kPairs, kSplit>;
+  auto kernel = i8d::gemm_i8_decode_kernel<kSwiglu, kPairs, kSplit, kFused>;
   static thread_local int configured_device = -1;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return set_error(SMB_ERR_CUDA, "cudaGetDevice failed");
@@ -437,10 +531,12 @@ int launch_i8_decode(const I8Launch& L, const i8d::Params& p, int ctas, int spli
 }  // namespace
 
 bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows) {
-  (void)N;
-  (void)K;
   if (groups == 1) {
+    // us here / best tiled kernel: 128 x 28672 x 8192 43 / 56, 128 x 4096 x 4096 11.3 / 14.1, 128 x 1024 x 8192
+    // 9.6 / 16.5, but 64 x 8192 x 2048 9.3 / 8.2: a short K loop over enough 128-wide tiles for most clusters
+    // leaves little to gain over 64 rows.
     if (M > 128 && !force) return false;
+    if (M >= 64 && N >= 8192 && K <= 2048 && !force) return false;
     *chunk = M >= 128 ? 128 : (M + 15) / 16 * 16;
     *box_rows = *chunk;
     return true;
@@ -455,10 +551,38 @@ bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int
   return true;
 }
 
+namespace {
+
+// K split: as many CTAs per tile as SMs are free, at least two K blocks each.  (As many as fill both places of
+// every SM: 1 x 4096 x 4096 7.5 instead of 7.1 us, 128 x 4096 x 4096 12.7 instead of 11.3.)
+int k_split(long long tiles, int K, int sms, int* kb_per) {
+  const int num_kb = (K + i8d::kBlockK - 1) / i8d::kBlockK;
+  int split = 1;
+  while (split < i8d::kMaxSplit && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
+  *kb_per = (num_kb + split - 1) / split;
+  return (num_kb + *kb_per - 1) / *kb_per;
+}
+
+template <bool kFused>
+int launch_form(const I8Launch& L, const i8d::Params& p, int ctas, int split, cudaStream_t stream) {
+  const bool pairs = L.ldd % 2 == 0 && reinterpret_cast<uintptr_t>(L.d) % 4 == 0 && L.tma_store;
+  if (L.swiglu)
+    return split > 1 ? launch_i8_decode<true, true, true, kFused>(L, p, ctas, split, stream)
+                     : launch_i8_decode<true, true, false, kFused>(L, p, ctas, split, stream);
+  if (pairs)
+    return split > 1 ? launch_i8_decode<false, true, true, kFused>(L, p, ctas, split, stream)
+                     : launch_i8_decode<false, true, false, kFused>(L, p, ctas, split, stream);
+  return split > 1 ? launch_i8_decode<false, false, true, kFused>(L, p, ctas, split, stream)
+                   : launch_i8_decode<false, false, false, kFused>(L, p, ctas, split, stream);
+}
+
+}  // namespace
+
 int i8_decode_launch(const I8Launch& L, cudaStream_t stream) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return set_error(SMB_ERR_CUDA, "i8 decode: no current device");
+  const int all_sms = sms;
   if (L.max_clusters > 0 && sms > 2 * L.max_clusters) sms = 2 * L.max_clusters;
   i8d::Params p = {};
   p.M = L.M;
@@ -486,31 +610,40 @@ int i8_decode_launch(const I8Launch& L, cudaStream_t stream) {
   if (L.offsets != nullptr) chunks = L.M / L.chunk + (L.groups < L.M ? L.groups : L.M);
   const long long tiles = chunks * p.tiles_n;
   if (tiles > 0x7FFFFFFFLL) return set_error(SMB_ERR_UNSUPPORTED, "i8 decode: too many tiles");
-  const int num_kb = (L.K + i8d::kBlockK - 1) / i8d::kBlockK;
-  // K split: as many CTAs per tile as SMs are free, at least two K blocks each.
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
-  p.kb_per = (num_kb + split - 1) / split;
-  split = (num_kb + p.kb_per - 1) / p.kb_per;
+  const int split = k_split(tiles, L.K, L.x != nullptr ? all_sms : sms, &p.kb_per);   // as the plan decided
   long long ctas;
   if (split > 1) {
     ctas = tiles * split;
   } else {
-    // Equal shares: the CTAs that t = ceil(tiles / SMs) tiles each leave busy.
-    const long long per = (tiles + sms - 1) / sms;
+    // Two CTAs per SM, equal shares: the CTAs that t = ceil(tiles / slots) tiles each leave busy.  16 x 28672 x
+    // 8192 from bf16: 38.6 us with two CTAs per SM, 43.7 with one of the same size, 40.5 with one of twice
+    // the ring; 128 experts x 256 rows gated 63.5 / 65.9 / 65.9.
+    const int slots = 2 * sms;
+    const long long per = (tiles + slots - 1) / slots;
     ctas = (tiles + per - 1) / per;
-    if (L.offsets != nullptr && ctas < sms && tiles >= sms) ctas = sms;   // the bound says little about the count
+    if (L.offsets != nullptr && ctas < slots && tiles >= slots) ctas = slots;   // the bound says little about the count
   }
-  const bool pairs = L.ldd % 2 == 0 && reinterpret_cast<uintptr_t>(L.d) % 4 == 0 && L.tma_store;
-  const int c = static_cast<int>(ctas);
-  if (L.swiglu)
-    return split > 1 ? launch_i8_decode<true, true, true>(L, p, c, split, stream)
-                     : launch_i8_decode<true, true, false>(L, p, c, split, stream);
-  if (pairs)
-    return split > 1 ? launch_i8_decode<false, true, true>(L, p, c, split, stream)
-                     : launch_i8_decode<false, true, false>(L, p, c, split, stream);
-  return split > 1 ? launch_i8_decode<false, false, true>(L, p, c, split, stream)
-                   : launch_i8_decode<false, false, false>(L, p, c, split, stream);
+  if (L.x != nullptr) {
+    // The stages hold weights alone; behind the ring lie the codes of the CTA's K range.
+    p.x = L.x;
+    p.ldx = L.ldx;
+    p.chunk = p.box_rows = i8d::kFusedRows;
+    p.stage_bytes = i8d::kWBytes;
+    p.stages = (i8d::kRingBudget / 1024 - p.kb_per) * 1024 / i8d::kWBytes;
+    if (p.stages > i8d::kMaxStages) p.stages = i8d::kMaxStages;
+    return launch_form<true>(L, p, static_cast<int>(ctas), split, stream);
+  }
+  return launch_form<false>(L, p, static_cast<int>(ctas), split, stream);
+}
+
+bool i8_decode_fuses(const I8Launch& L, const void* x, long long ldx) {
+  if (!L.decode || L.offsets != nullptr || L.M > i8d::kFusedTokens || L.K % 8 != 0 || ldx % 8 != 0 ||
+      reinterpret_cast<uintptr_t>(x) % 16 != 0)
+    return false;
+  int kb_per = 0;
+  const int slots = device_cluster_slots();
+  k_split((L.N + i8d::kTileRows - 1) / i8d::kTileRows, L.K, slots > 0 ? 2 * slots : 148, &kb_per);
+  return kb_per <= i8d::kFusedMaxBlocks;
 }
 
 }  // namespace smb

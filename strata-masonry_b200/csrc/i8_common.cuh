@@ -29,6 +29,8 @@ struct I8Launch {
   int chunk;             // decode: rows of A per tile, a multiple of 16 up to 128
   int box_rows;          // decode: rows of A per TMA box
   bool weights_static;   // B and sb are not written by work that may still run on the stream
+  const uint16_t* x;     // decode: bf16 rows that the kernel quantises itself (i8_decode_fuses), else null
+  long long ldx;
   int* status;
 };
 
@@ -37,6 +39,7 @@ int i8_launch(const I8Launch& L, cudaStream_t stream);
 // Whether the decode kernel is taken for M rows in `groups` groups, with its chunk and box heights.
 bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows);
 int i8_decode_launch(const I8Launch& L, cudaStream_t stream);
+bool i8_decode_fuses(const I8Launch& L, const void* x, long long ldx);   // for plain plans fed with bf16 rows
 
 // Rows of `src` (bf16 or fp32) to int8 codes and one scale per row.  The next kernel on the stream may
 // start its prologue early.

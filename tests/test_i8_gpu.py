@@ -211,7 +211,8 @@ def test_i8_grouped_plan_follows_its_offsets(smb, cuda_device, mode):
 
 @pytest.mark.parametrize("flags_name", ["FLAG_NONE", "FLAG_WEIGHTS_STATIC"])
 @pytest.mark.parametrize("shape", [(1, 4096, 4096), (16, 4096, 2048), (100, 1000, 1056), (129, 300, 520), (700, 600, 1000),
-                                   (3, 130, 77), (64, 28672, 1024)])
+                                   (3, 130, 77), (64, 28672, 1024), (8, 28672, 1024), (5, 301, 8200), (7, 1000, 12296),
+                                   (2, 20000, 12288), (8, 8, 8), (1, 2048, 136)])
 def test_i8_plan_fed_with_bf16_activations(smb, cuda_device, shape, flags_name):
     torch = _torch()
     m, n, k = shape
@@ -235,6 +236,42 @@ def test_i8_plan_fed_with_bf16_activations(smb, cuda_device, shape, flags_name):
     plan.check()
     smb.gemm.quantize_i8_bf16_device(x, codes, scales, m, k)
     _check(torch, d, _sums(torch, codes, b, k), scales, sb)
+
+
+@pytest.mark.parametrize("m", [1, 6, 8, 9])
+def test_i8_gated_plan_fed_with_bf16_activations(smb, cuda_device, m):
+    torch = _torch()
+    n, k = 1552, 2048
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    x = torch.randn(m, k + 8, generator=g, device="cuda").bfloat16()
+    if m > 2:
+        x[1] = 0.0
+    b = _codes(torch, n, k, 7)
+    sb = torch.full((n,), 0.05 / 74, device="cuda")
+    d = torch.full((m, n // 2), float("nan"), device="cuda", dtype=torch.bfloat16)
+    plan = smb.gemm.I8Plan.from_bf16_activations(x, b, sb, d, m, n, k, ldx=k + 8, ldb=b.shape[1],
+                                                 flags=smb.capi.FLAG_EPILOGUE_SWIGLU | smb.capi.FLAG_WEIGHTS_STATIC)
+    plan.run()
+    plan.check()
+    codes, scales = torch.zeros(m, k, device="cuda", dtype=torch.int8), torch.zeros(m, device="cuda")
+    smb.gemm.quantize_i8_bf16_device(x, codes, scales, m, k, ld_src=k + 8)
+    _check_gated(torch, d, _sums(torch, codes, b, k), scales, sb)
+
+
+def test_i8_nan_token_in_the_fused_quantiser(smb, cuda_device):
+    torch = _torch()
+    m, n, k = 4, 300, 1024
+    x = torch.randn(m, k, device="cuda").bfloat16()
+    x[2, 1000] = float("inf")
+    b, sb = _codes(torch, n, k, 1), _scales(torch, n, 2)
+    d = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+    plan = smb.gemm.I8Plan.from_bf16_activations(x, b, sb, d, m, n, k)
+    assert "fused" in plan.describe()
+    plan.run()
+    plan.check()
+    bad = torch.isnan(d.float())
+    assert bool(bad[2].all()) and int(bad.sum()) == n
 
 
 def test_i8_two_plans_on_two_streams(smb, cuda_device):
