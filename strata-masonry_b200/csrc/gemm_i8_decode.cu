@@ -541,12 +541,13 @@ bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int
     *box_rows = *chunk;
     return true;
   }
-  // Chunks of twice the average, so that few experts need two; above 96 rows per expert the 256-row
-  // tiles win.  64 experts of 2048 x 2048, us here (chunk) / tiled: 8 rows each 47.0 (16) / 56.1, 24 46.6
-  // (64) / 58.4, 48 47.6 (64) / 59.8, 95 55.8 (128) / 60.2, 127 75.1 (128) / 61.8.
+  // Small chunks keep the stages small and the ring deep; large ones keep experts in one chunk.  us with
+  // chunks of 16 / 32 / 64 / 128: 128 experts of 1536 x 2048 with 4 rows on average 61.9 / 65.1 / 66.2 / 69.0, 12
+  // rows 67.7 / 66.7 / 67.7 / 69.9, 48 rows - / 73.9 / 69.4 / 73.1, 95 rows - / - / 85.5 / 75.8.  Above 96 rows the
+  // 256-row tiles win: 64 experts of 2048 x 2048, 95 rows 52.4 here and 58.6 tiled, 127 rows 60.5 and 59.2.
   const int average = (M + groups - 1) / groups;
   if (average > 96 && !force) return false;
-  *chunk = average <= 8 ? 16 : (average <= 16 ? 32 : (average <= 48 ? 64 : 128));
+  *chunk = average <= 8 ? 16 : (average <= 16 ? 32 : (average <= 64 ? 64 : 128));
   *box_rows = 16;
   return true;
 }
