@@ -198,33 +198,6 @@ __device__ __forceinline__ void quantize_tokens(const Params& p, int kb0, int kb
     asm volatile("st.shared.f32 [%0], %1;" ::"r"(sa + 4u * r), "f"(rs.bad ? __uint_as_float(0x7FC00000u) : rs.scale) : "memory");
 }
 
-// Two tokens (rows m, m + 1 of D) of this lane's channel n, already scaled.  Neighbouring lanes trade
-// halves, so that even lanes write two channels of row m and odd lanes two of row m + 1; with the gated
-// epilogue the two are up and gate of one output.
-template <bool kSwiglu, bool kPairs>
-__device__ __forceinline__ void store_pair(const Params& p, long long m, int valid, int n, float z0, float z1) {
-  if (!kSwiglu && !kPairs) {
-    if (n < p.N) {
-      if (valid > 0) p.d_ptr[m * p.ldd + n] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(z0), 0u) & 0xFFFFu);
-      if (valid > 1) p.d_ptr[(m + 1) * p.ldd + n] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(z1), 0u) & 0xFFFFu);
-    }
-    return;
-  }
-  const bool odd = n & 1;
-  const float other = __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
-  const float lo = odd ? other : z0, hi = odd ? z1 : other;
-  const int n0 = n & ~1;
-  if (valid <= (odd ? 1 : 0) || n0 >= p.N) return;
-  uint16_t* row = p.d_ptr + (m + (odd ? 1 : 0)) * p.ldd;
-  if (kSwiglu) {
-    row[n0 >> 1] = static_cast<uint16_t>(pack_bf16x2(__float_as_uint(silu_mul(hi, lo)), 0u) & 0xFFFFu);
-  } else {
-    const uint32_t v = pack_bf16x2(__float_as_uint(lo), __float_as_uint(hi));
-    if (n0 + 1 < p.N) *reinterpret_cast<uint32_t*>(row + n0) = v;
-    else row[n0] = static_cast<uint16_t>(v & 0xFFFFu);
-  }
-}
-
 // kSplit: the CTAs of a cluster share the K loop of ONE tile (the grid has a cluster for every tile).
 // kFused: bf16 tokens (at most 4, a plain product), codes and scales made here.
 template <bool kSwiglu, bool kPairs, bool kSplit, bool kFused>
@@ -432,13 +405,8 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         } else {
           const float scale = sa;
           sa = token_scale(scales, tile, c0 + 32 + (lane & 15));
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const int c = c0 + i;
-            const float s0 = __shfl_sync(0xffffffffu, scale, i), s1 = __shfl_sync(0xffffffffu, scale, i + 1);
-            if (c < tile.rows)
-              store_pair<kSwiglu, kPairs>(p, tile.row0 + c, tile.rows - c, n, scale_i32(v[i], s0, sb), scale_i32(v[i + 1], s1, sb));
-          }
+          store_tokens<16, kSwiglu, kPairs>(v, scale, sb, p.d_ptr + static_cast<long long>(tile.row0 + c0) * p.ldd, p.ldd, p.N,
+                                            tile.rows - c0, n);
         }
       }
       tc_fence_before_sync();
@@ -475,12 +443,7 @@ gemm_i8_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         for (int q = 0; q < kMaxSplit; ++q)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum[i] += part[q][i];
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const float s0 = __shfl_sync(0xffffffffu, sa, i), s1 = __shfl_sync(0xffffffffu, sa, i + 1);
-          if (c + i < end)
-            store_pair<kSwiglu, kPairs>(p, tile.row0 + c + i, end - c - i, n, scale_i32(sum[i], s0, sb), scale_i32(sum[i + 1], s1, sb));
-        }
+        store_tokens<4, kSwiglu, kPairs>(sum, sa, sb, p.d_ptr + static_cast<long long>(tile.row0 + c) * p.ldd, p.ldd, p.N, end - c, n);
       }
     }
     cluster_sync_all();   // partial sums stay until every CTA has read them

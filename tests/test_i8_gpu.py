@@ -170,14 +170,16 @@ GROUPS = [((300, 0, 77, 512, 1), 384, 256), ((0, 0, 1), 130, 100), ((1,) * 40, 2
 
 
 @pytest.mark.parametrize("case", GROUPS, ids=lambda c: f"{len(c[0])}x{c[1]}x{c[2]}")
-@pytest.mark.parametrize("mode", ["plain", "gated", "no_decode", "wide", "plain_store", "decode", "decode_gated"])
+@pytest.mark.parametrize("mode", ["plain", "gated", "no_decode", "wide", "plain_store", "decode", "decode_gated", "tiled_gated",
+                                  "tiled_plain_store"])
 def test_i8_grouped_ragged(smb, cuda_device, case, mode):
     torch = _torch()
     sizes, n, k = case
     c = smb.capi
     flags = {"plain": 0, "gated": c.FLAG_EPILOGUE_SWIGLU, "no_decode": c.FLAG_NO_DECODE,
              "wide": c.FLAG_NO_DECODE | c.FLAG_TILE_N_512, "plain_store": c.FLAG_FORCE_PLAIN_STORE,
-             "decode": c.FLAG_DECODE_SINGLE, "decode_gated": c.FLAG_DECODE_SINGLE | c.FLAG_EPILOGUE_SWIGLU}[mode]
+             "tiled_gated": c.FLAG_NO_DECODE | c.FLAG_EPILOGUE_SWIGLU,
+             "tiled_plain_store": c.FLAG_NO_DECODE | c.FLAG_FORCE_PLAIN_STORE, "decode": c.FLAG_DECODE_SINGLE, "decode_gated": c.FLAG_DECODE_SINGLE | c.FLAG_EPILOGUE_SWIGLU}[mode]
     if mode.endswith("gated"):
         n = (n + 15) // 16 * 16
     plan, ends, offsets, a, sa, b, sb, d = _run_grouped(smb, torch, sizes, n, k, flags, slack=40)
