@@ -485,7 +485,9 @@ int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, co
 
 /* ------------------------------------------------------------------------------------
  * Routing to experts and the rows of the grouped GEMMs.  All on the device, stream-ordered, without
- * host synchronisation, atomics or allocation: a whole expert layer can be captured in a CUDA graph.
+ * host synchronisation, atomics, workspaces or allocation: a whole expert layer can be captured in a
+ * CUDA graph, and calls on different streams do not disturb one another.  Run them with the device of
+ * the buffers current.
  * tokens == 0 is a valid, empty call (pointers to its empty arrays may be NULL).  No reference counterpart (its tree has the tile map of a
  * grouped GEMM only, composites/83_grouped_gemm_tile_map.cuh:71-101).
  * ---------------------------------------------------------------------------------- */
@@ -499,7 +501,7 @@ int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, co
  * best expert first, ties to the lowest index.  Compared are p + bias (bias: [experts] fp32 or NULL; it
  * takes no part in the weights), without a bias the logits.  With top_groups < n_groups only experts of
  * the top_groups best of n_groups equal runs of experts can be chosen.  weight = scale * p, or with
- * RENORM scale * p / sum.  Experts whose logit is -inf or NaN (or bias -inf) are closed; where fewer
+ * RENORM scale * p / sum.  ids and weights are contiguous.  Experts whose logit is -inf or NaN (or bias -inf) are closed; where fewer
  * than top_k are open the remaining slots hold id -1 and weight 0 (so a padding row of -inf routes
  * nowhere).  Up to 512 experts, top_k <= 32, n_groups <= 32. */
 int smb_moe_route_device(const void* logits, int dtype, int64_t ld, const float* bias, int tokens, int experts,
@@ -525,8 +527,9 @@ int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int top_k, int g
                             int64_t max_rows, int32_t* offsets, int32_t* row_of_slot, int32_t* slot_of_row,
                             int32_t* mtile_group, void* stream);
 /* Row row_of_slot[t, j] of the output becomes row t of x, as bf16 or quantised (rule of
- * smb_quantize_i8_bf16_device, quantised once per token).  Rows that no slot names are left alone;
- * entries outside [0, max_rows) are skipped.  The gradient of x is smb_moe_combine_device without
+ * smb_quantize_i8_bf16_device, quantised once per token).  row_of_slot is contiguous and names a row at
+ * most once (as smb_moe_dispatch_device writes it).  Rows that no slot names are left alone; entries
+ * outside [0, max_rows) are skipped.  The gradient of x is smb_moe_combine_device without
  * weights. */
 int smb_moe_gather_bf16_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens,
                                int top_k, int width, int64_t max_rows, uint16_t* out, int64_t ld_out,

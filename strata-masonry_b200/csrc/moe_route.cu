@@ -821,6 +821,8 @@ extern "C" int smb_moe_route_device(const void* logits, int dtype, int64_t ld, c
                            SMB_ROUTE_SIGMOID | SMB_ROUTE_RENORM | SMB_ROUTE_GROUP_TOP2))
     return rc;
   if (tokens != 0 && (ids == nullptr || weights == nullptr)) return set_error(SMB_ERR_INVALID, "route: null output");
+  for (const void* q : {static_cast<const void*>(bias), static_cast<const void*>(ids), static_cast<const void*>(weights)})
+    if (reinterpret_cast<uintptr_t>(q) % 4 != 0) return set_error(SMB_ERR_INVALID, "route: bias, ids and weights must be 4-byte aligned");
   if (n_groups < 1 || n_groups > kMaxRouteGroups || experts % n_groups != 0)
     return set_error(SMB_ERR_INVALID, "route: %d groups must divide %d experts and be at most %d", n_groups, experts,
                      kMaxRouteGroups);
@@ -846,6 +848,9 @@ extern "C" int smb_moe_route_backward_device(const void* logits, int dtype, int6
     return rc;
   if (tokens != 0 && (ids == nullptr || grad_weights == nullptr || grad_logits == nullptr))
     return set_error(SMB_ERR_INVALID, "route backward: null pointer");
+  for (const void* q : {static_cast<const void*>(ids), static_cast<const void*>(grad_weights)})
+    if (reinterpret_cast<uintptr_t>(q) % 4 != 0)
+      return set_error(SMB_ERR_INVALID, "route backward: ids and gradients must be 4-byte aligned");
   if (ld_grad < experts) return set_error(SMB_ERR_INVALID, "route backward: gradient pitch smaller than the number of experts");
   if (reinterpret_cast<uintptr_t>(grad_logits) % (dtype == SMB_DTYPE_BF16 ? 2 : 4) != 0)
     return set_error(SMB_ERR_INVALID, "route backward: gradient is not aligned to its type");

@@ -122,7 +122,8 @@ def test_i8_null_handles_and_host_refusals(smb):
     (dict(top_k=33), "top_k"), (dict(experts=4, n_groups=1, top_groups=1, top_k=5), "top_k"), (dict(ld=63), "pitch"),
     (dict(n_groups=3), "groups"), (dict(n_groups=64), "groups"), (dict(n_groups=0), "groups"), (dict(top_groups=0), "top_groups"),
     (dict(top_groups=9), "top_groups"), (dict(top_groups=1, top_k=9), "open groups"), (dict(flags=8), "flags"),
-    (dict(ids=None), "null output"), (dict(weights=None), "null output"),
+    (dict(ids=None), "null output"), (dict(weights=None), "null output"), (dict(ids=ODD), "4-byte"),
+    (dict(weights=C.c_void_p(0x10002)), "4-byte"), (dict(bias=C.c_void_p(0x10002)), "4-byte"),
 ])
 def test_route_refusals(smb, change, text):
     args = dict(logits=P, dtype=0, ld=64, bias=None, tokens=8, experts=64, top_k=4, n_groups=8, top_groups=4, flags=0, scale=1.0,
