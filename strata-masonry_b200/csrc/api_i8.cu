@@ -135,6 +135,8 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
   if (rc == SMB_OK && L.x == nullptr)
     rc = encode_tmap_2d(&L.tmap_a, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, L.decode ? L.box_rows : 128, 128,
                         true);
+  if (rc == SMB_OK && L.offsets != nullptr && !L.decode)
+    rc = encode_tmap_2d(&L.tmap_a32, a, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, g.M, g.K, lda, 32, 128, true);
   if (rc == SMB_OK)
     rc = encode_tmap_2d(&L.tmap_b, g.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, static_cast<uint64_t>(g.groups) * g.N, g.K, g.ldb,
                         L.decode ? 128 : L.tile_n / 2, 128, true);

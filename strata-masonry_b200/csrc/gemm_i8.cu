@@ -124,8 +124,9 @@ __device__ __forceinline__ RowTile find_row_tile(const Params& p, const uint16_t
 
 template <int TN, int NB, int kStore>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-               const __grid_constant__ CUtensorMap tmap_d, const __grid_constant__ Params p) {
+gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a32,
+               const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_d,
+               const __grid_constant__ Params p) {
   using C = Cfg<TN, NB>;
   constexpr bool kTmaStore = (kStore != kStorePlain);
   constexpr bool kSwiglu = (kStore == kStoreSwiglu);
@@ -198,8 +199,9 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
       tile_coords(t, tiles_m, p.tiles_n, group_m, tm, tn);
       RowTile rt = {tm * 256, p.M, 0};
       if (grouped) rt = find_row_tile(p, table, tm, lane);
-      // A tile reads on past the end of its group (rows it never stores) and past N.
+      // B is read on past N (columns that are never stored).
       const int row_a = rt.row0 + static_cast<int>(rank) * kBlockM;
+      const bool ragged = grouped && row_a + kBlockM > rt.row_end;   // the group ends in this CTA's half
       const int row_b = rt.group * p.N + tn * C::kTileN + static_cast<int>(rank) * (TN / 2);
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!mbar_wait(empty_bar(s), ph ^ 1u)) {
@@ -211,7 +213,16 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
         const uint32_t dst_a = ring_base + s * C::kStageBytes;
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * C::kStageBytes);
-          tma_load_2d_pair_hint(dst_a, &tmap_a, bar, kb * kBlockK, row_a, pol);
+          if (ragged) {
+            // Rows of other groups would be multiplied in vain; in steps of 32 they are fetched from beyond
+            // the end of A instead, as zeros, which cost the tensor cores less power and L2 nothing.
+#pragma unroll
+            for (int q = 0; q < kBlockM; q += 32)
+              tma_load_2d_pair_hint(dst_a + q * kBlockK, &tmap_a32, bar, kb * kBlockK, row_a + q < rt.row_end ? row_a + q : p.M,
+                                    pol);
+          } else {
+            tma_load_2d_pair_hint(dst_a, &tmap_a, bar, kb * kBlockK, row_a, pol);
+          }
 #pragma unroll
           for (int h = 0; h < NB; ++h)
             tma_load_2d_pair_hint(dst_a + kABytes + h * C::kBBytes, &tmap_b, bar, kb * kBlockK, row_b + h * TN, pol);
@@ -397,7 +408,7 @@ int launch_i8(const I8Launch& L, cudaStream_t stream) {
   pdl.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &pdl;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L.tmap_a, L.tmap_b, L.tmap_d, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, L.tmap_a, L.tmap_a32, L.tmap_b, L.tmap_d, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "i8 GEMM launch");
   return SMB_OK;

@@ -12,6 +12,7 @@ constexpr int kI8MaxK = 131071;          // 128 * 128 * K stays below 2^31: int3
 
 struct I8Launch {
   CUtensorMap tmap_a, tmap_b, tmap_d;
+  CUtensorMap tmap_a32;   // grouped tiled kernel: A in boxes of 32 rows
   int M, N, K;           // M: rows of A (grouped: upper bound of the rows in use)
   int tile_n;            // tiled kernel: width of one N sub-block, 128 or 256
   int sub_blocks;        // 1, or 2 (256 x 512 tiles)
