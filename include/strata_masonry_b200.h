@@ -485,7 +485,7 @@ int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, co
 
 /* ------------------------------------------------------------------------------------
  * Routing to experts and the rows of the grouped GEMMs.  All on the device, stream-ordered, without
- * host synchronisation, atomics, workspaces or allocation: a whole expert layer can be captured in a
+ * host synchronisation, workspaces or allocation, and give the same bits every time: a whole expert layer can be captured in a
  * CUDA graph, and calls on different streams do not disturb one another.  Run them with the device of
  * the buffers current.
  * tokens == 0 is a valid, empty call (pointers to its empty arrays may be NULL).  No reference counterpart (its tree has the tile map of a

@@ -7,7 +7,8 @@
 //   combine    y[t] = sum_j weights[t, j] * rows[row_of_slot[t, j]], and its gradients
 //
 // A slot that goes nowhere (id outside [0, experts)) has row -1 and is skipped everywhere; rows that no
-// slot names are never written.  No atomics: the order of every sum and of the rows is fixed.
+// slot names are never written.  The order of every sum and of the rows is fixed (the only atomics are
+// integer counts in shared memory).
 #include "i8_common.cuh"
 #include "ptx.cuh"
 #include "quant_i8.cuh"
@@ -55,6 +56,18 @@ constexpr int kHeldIds = 8;
 
 __device__ __forceinline__ int clean_id(int e, int groups) { return e >= 0 && e < groups ? e : -1; }
 
+// Lanes with this lane's id, from a ballot per bit of it (`bits` cover every id and the -1 of dropped slots).
+// match.any takes longer, and longer still the more ids differ: 65536 slots of 64 groups 24 us with it.
+__device__ __forceinline__ unsigned same_id(int e, int bits) {
+  unsigned same = kFull;
+  for (int b = 0; b < bits; ++b) {
+    const bool bit = (e >> b) & 1;
+    const unsigned set = __ballot_sync(kFull, bit);
+    same &= bit ? set : ~set;
+  }
+  return same;
+}
+
 template <bool kCluster>
 __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) {
   extern __shared__ int sm[];
@@ -96,9 +109,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
     for (int i = 0; i < kHeldIds; ++i) {
       if (s0 + i * 32 >= hi) break;
       const int e = clean_id(held[i], G);
-      const unsigned same = __match_any_sync(kFull, e);
-      if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-      __syncwarp();
+      if (e >= 0) atomicAdd(mine + e, 1);   // the warp's own words; a count does not depend on the order
     }
   }
   __syncthreads();
@@ -155,6 +166,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   const int others = lane < warps ? warp_sums[lane] : 0;
   int base = __reduce_add_sync(kFull, lane < warp ? others : 0) + inclusive - sum;
   const int used = __reduce_add_sync(kFull, others);
+  const int id_bits = 32 - __clz(G);   // G < 2^bits, so the low bits of -1 are no id either
   for (int e = e_lo; e < e_hi; ++e) {
     total[e] = base;                  // first row of the group, from here on
     start[e] += base;
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
       const int s = s0 + i * 32 + lane;
       if (s0 + i * 32 >= hi) break;
       const int e = clean_id(held[i], G);
-      const unsigned same = __match_any_sync(kFull, e);
+      const unsigned same = same_id(e, id_bits);
       const int row = e >= 0 ? start[e] + mine[e] + __popc(same & ((1u << lane) - 1u)) : -1;
       __syncwarp();
       if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
