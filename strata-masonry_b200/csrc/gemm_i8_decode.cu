@@ -1,5 +1,7 @@
 // int8 GEMM for few rows per weight matrix (decode batches, experts with a handful of tokens): bound by
-// reading B once.  Same result, bit for bit, as gemm_i8.cu.
+// reading B once.  Same result, bit for bit, as gemm_i8.cu.  Measured: 16 x 28672 x 8192 with its quantiser 38 us
+// (6.2 TB/s), 128 experts x 256 rows (1536 x 2048 each, gated) 63 us (6.4 TB/s), DRAM reads the operands once
+// (ncu: 235.2 and 404.0 MB).
 //
 // The operands swap roles: 128 rows of B (output channels) fill the rows of a 1-CTA tcgen05.mma and up
 // to 128 rows of A (tokens) its columns, so the instruction does no more work than the tokens need and a

@@ -101,46 +101,59 @@ __host__ __device__ inline RowScale row_scale(float amax, bool finite) {
   return r;
 }
 
-// One row by `kThreads` threads of a CTA (32: a warp, no barrier; more: `red` holds one word per warp
-// of the CTA, and the CTA's threads belong to one row).  `store8(k, codes)` and `store1(k, code)`
-// receive the codes, after a barrier of the row's threads; returns the row's scale.  kVecs vectors per thread stay in registers between the
-// two passes, longer rows are read again (from L2).
-template <bool kBf16, int kThreads, int kVecs, bool kAligned, class Store8, class Store1>
-__device__ __forceinline__ float quantize_row(const void* row, int K, int tid, uint32_t* red, Store8 store8,
+constexpr int kHeldVecs = 4;      // vectors of a row that a thread keeps between the two passes
+constexpr int kMaxRowWarps = 16;
+
+// Threads that share a row of K elements as a CTA of their own.  Many rows: as few as hold the row in registers,
+// since few threads with four vectors each keep more rows in flight than many with one (4095 x 4160 bf16 10.0
+// against 12.2 us).  Few rows: as many as there are vectors, for the shortest way through one row (rows
+// of 4096 for 16 tokens to 8 experts each, in the chain that sorts and sums them: 6.3 against 7.1 us).
+inline int row_threads(int64_t K, int64_t rows) {
+  const int vecs = rows <= 4 * 148 ? 1 : kHeldVecs;
+  int64_t t = (K / 8 + vecs - 1) / vecs;
+  t = (t + 31) / 32 * 32;
+  return static_cast<int>(t < 64 ? 64 : (t > kMaxRowWarps * 32 ? kMaxRowWarps * 32 : t));
+}
+
+// One row by `threads` threads: a warp (kWarp, no CTA barrier), or the whole CTA, `red` then holding a word
+// per warp.  `store8(k, codes)` and `store1(k, code)` receive the codes, after a barrier of the row's
+// threads; returns the row's scale.  Rows too long for the registers are read again (from L2).
+template <bool kBf16, bool kWarp, bool kAligned, class Store8, class Store1>
+__device__ __forceinline__ float quantize_row(const void* row, int K, int tid, int threads, uint32_t* red, Store8 store8,
                                               Store1 store1) {
   const int nvec = kAligned ? K / 8 : 0;
-  Vec<kBf16> held[kVecs];
+  Vec<kBf16> held[kHeldVecs];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int v = tid + i * kThreads;
+  for (int i = 0; i < kHeldVecs; ++i) {
+    const int v = tid + i * threads;
     if (v < nvec) held[i] = load_vec<kBf16>(row, static_cast<int64_t>(v) * 8);
   }
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i)
-    if (tid + i * kThreads < nvec) m = abs_max_bits<kBf16>(held[i], m);
-  for (int v = tid + kVecs * kThreads; v < nvec; v += kThreads)
+  for (int i = 0; i < kHeldVecs; ++i)
+    if (tid + i * threads < nvec) m = abs_max_bits<kBf16>(held[i], m);
+  for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
     m = abs_max_bits<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), m);
-  for (int k = nvec * 8 + tid; k < K; k += kThreads)
+  for (int k = nvec * 8 + tid; k < K; k += threads)
     m = max(m, __float_as_uint(load_one<kBf16>(row, k)) & 0x7FFFFFFFu);
   m = __reduce_max_sync(0xffffffffu, m);
   __syncwarp();   // what the caller put into shared memory is there for store8 / store1
-  if (kThreads > 32) {
+  if (!kWarp) {
     if ((tid & 31) == 0) red[tid >> 5] = m;
     __syncthreads();
-    m = red[tid & (kThreads / 32 - 1)];
+    m = (tid & 31) < (threads >> 5) ? red[tid & 31] : 0u;
     m = __reduce_max_sync(0xffffffffu, m);
   }
   const RowScale rs = row_scale(__uint_as_float(m), m < 0x7F800000u);
   const float inv = rs.inv;
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const int v = tid + i * kThreads;
+  for (int i = 0; i < kHeldVecs; ++i) {
+    const int v = tid + i * threads;
     if (v < nvec) store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(held[i], inv));
   }
-  for (int v = tid + kVecs * kThreads; v < nvec; v += kThreads)
+  for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
     store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), inv));
-  for (int k = nvec * 8 + tid; k < K; k += kThreads)
+  for (int k = nvec * 8 + tid; k < K; k += threads)
     store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(load_one<kBf16>(row, k), inv) & 0xFFu));
   return rs.bad ? __uint_as_float(0x7FC00000u) : rs.scale;
 }
