@@ -37,8 +37,8 @@ constexpr int kBarBytes = 384;
 constexpr int kFusedTokens = 4;       // most tokens quantised in the kernel
 constexpr int kFusedRows = 8;         // rows of their codes in shared memory: the smallest N of the MMA
 // K blocks of codes (1 KB each) beside the ring, which keeps five stages.  us with the quantiser inside / as
-// a launch of its own, 1, 4 and 8 tokens: 4096 x 4096 (8 blocks per CTA) 7.1 / 8.3, 7.6 / 8.4, 8.5 / 8.4;
-// 28672 x 8192 (64 blocks, two stages left) 44.6 / 39.9.
+// a launch of its own, 1 and 4 tokens: 4096 x 4096 (8 blocks per CTA) 6.6 / 7.6, 7.3 / 7.8 (8 tokens, before the last
+// steps: 8.5 / 8.4); 28672 x 8192 (64 blocks, two stages left) 44.6 / 39.9.
 constexpr int kFusedMaxBlocks = 24;
 constexpr int kTableBytes = (kI8MaxGroups + 8) * 4;
 // Half of an SM's shared memory, and at most half of its tensor memory: two CTAs share an SM, so the next
@@ -573,7 +573,7 @@ bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int
 namespace {
 
 // K split: as many CTAs per tile as SMs are free, at least two K blocks each.  (As many as fill both places of
-// every SM: 1 x 4096 x 4096 7.5 instead of 7.1 us, 128 x 4096 x 4096 12.7 instead of 11.3.)
+// every SM: 1 x 4096 x 4096 from bf16 7.3 instead of 6.6 us, 128 x 4096 x 4096 12.7 instead of 11.3.)
 int k_split(long long tiles, int K, int sms, int* kb_per) {
   const int num_kb = (K + i8d::kBlockK - 1) / i8d::kBlockK;
   int split = 1;
