@@ -433,14 +433,15 @@ int smb_fp4_host_ctx_create_sharded(smb_fp4_host_ctx** ctx, int M, int n_local, 
  *   D[m,n] = bf16_rne( (float(sum_k A[m,k] B[n,k]) * sa[m]) * sb[n] ),  the sum exact in int32.
  * A [M,K] and B [N,K] are int8, row-major, row pitches multiples of 16 bytes, base pointers 16-byte
  * aligned; sa [M] and sb [N] are fp32; D is bf16 row-major with the store rules of the BF16 GEMM.
- * Any M, N >= 1 and 1 <= K <= 131071 (the int32 sum of 131072 products could wrap).  No reference
+ * Any M, N from 1 to 2^30 and 1 <= K <= 131071 (the int32 sum of 131072 products could wrap).  No reference
  * counterpart: its int8 path is not part of the dense GEMM tree.
  * ---------------------------------------------------------------------------------- */
 
 /* Per-row quantiser, for activations (rows are tokens) and weights (rows are output channels):
  *   amax = max(max|x|, 2^-100), scale = amax / 127, code = round_half_even(x * (127 / amax)),
  * every operation in fp32, so all forms agree bit for bit.  A row that holds an infinity or a NaN
- * gets codes 0 and scale NaN.  K codes per row are written, the rest of the pitch is left alone. */
+ * gets codes 0 and scale NaN.  K (at most 2^30) codes per row are written, the rest of the pitch is left
+ * alone. */
 int smb_quantize_i8_device(const float* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
                            int64_t rows, int64_t K, void* stream);
 int smb_quantize_i8_bf16_device(const uint16_t* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes,
@@ -449,9 +450,9 @@ int smb_quantize_i8_host(const float* src, int64_t ld_src, int8_t* codes, int64_
                          int64_t rows, int64_t K);
 
 /* Plans as for the BF16 GEMM.  Flags: SMB_FLAG_FORCE_PLAIN_STORE, _TILE_N_128 / _256 / _512,
- * _NO_DECODE, _DECODE_SINGLE (force the kernel for few rows), _EPILOGUE_SWIGLU (rows of B interleaved, even = up, odd = gate, D [M, N / 2] =
- * bf16(silu(gate) * up) of the scaled sums, silu accurate to fp32), _WEIGHTS_STATIC; others are
- * refused. */
+ * _NO_DECODE, _DECODE_SINGLE (force the kernel for few rows), _EPILOGUE_SWIGLU (rows of B interleaved,
+ * even = up, odd = gate, D [M, N / 2] = bf16(silu(gate) * up) of the scaled sums, silu accurate to fp32 and
+ * zero below a gate of -87, where it is smaller than 2^-119), _WEIGHTS_STATIC; others are refused. */
 typedef struct smb_i8_plan smb_i8_plan;
 int smb_i8_plan_create(smb_i8_plan** plan, const void* a, const float* sa, const void* b, const float* sb,
                        void* d, int M, int N, int K, int64_t lda, int64_t ldb, int64_t ldd, unsigned flags);
@@ -485,11 +486,11 @@ int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, co
 
 /* ------------------------------------------------------------------------------------
  * Routing to experts and the rows of the grouped GEMMs.  All on the device, stream-ordered, without
- * host synchronisation, workspaces or allocation, and give the same bits every time: a whole expert layer can be captured in a
- * CUDA graph, and calls on different streams do not disturb one another.  Run them with the device of
- * the buffers current.
- * tokens == 0 is a valid, empty call (pointers to its empty arrays may be NULL).  No reference counterpart (its tree has the tile map of a
- * grouped GEMM only, composites/83_grouped_gemm_tile_map.cuh:71-101).
+ * host synchronisation, workspaces or allocation, and the same bits every time: a whole expert layer can
+ * be captured in a CUDA graph, and calls on different streams do not disturb one another.  Run them with
+ * the device of the buffers current.  tokens == 0 is a valid, empty call (pointers to its empty arrays may
+ * be NULL).  No reference counterpart (its tree has the tile map of a grouped GEMM only,
+ * composites/83_grouped_gemm_tile_map.cuh:71-101).
  * ---------------------------------------------------------------------------------- */
 #define SMB_DTYPE_F32 0
 #define SMB_DTYPE_BF16 1

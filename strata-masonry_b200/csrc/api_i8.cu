@@ -43,6 +43,8 @@ int check_args(const I8Args& g) {
   if (g.b == nullptr || g.sb == nullptr || g.d == nullptr) return set_error(SMB_ERR_INVALID, "i8 plan: null operand pointer");
   if (g.M <= 0 || g.N <= 0 || g.K <= 0)
     return set_error(SMB_ERR_INVALID, "i8 plan: dimensions must be positive (M=%d N=%d K=%d)", g.M, g.N, g.K);
+  if (g.M > kI8MaxExtent || g.N > kI8MaxExtent)
+    return set_error(SMB_ERR_UNSUPPORTED, "i8 plan: M=%d N=%d above %d", g.M, g.N, kI8MaxExtent);
   if (g.K > kI8MaxK)
     return set_error(SMB_ERR_UNSUPPORTED, "i8 plan: K=%d above %d, where an int32 sum could wrap", g.K, kI8MaxK);
   if (g.flags & ~kKnownFlags) return set_error(SMB_ERR_UNSUPPORTED, "i8 plan: flags 0x%x have no int8 form", g.flags & ~kKnownFlags);

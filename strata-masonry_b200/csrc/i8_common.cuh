@@ -8,6 +8,7 @@ namespace smb {
 
 constexpr int kI8MaxGroups = 512;        // grouped plans: entries of the kernels' row-tile table
 constexpr int kI8MaxRows = 8 << 20;      // ... whose 16-bit counts hold 65535 tiles of 256 rows
+constexpr int kI8MaxExtent = 1 << 30;    // M and N: tiles that end behind them stay within 31 bits
 constexpr int kI8MaxK = 131071;          // 128 * 128 * K stays below 2^31: int32 sums never wrap
 
 struct I8Launch {

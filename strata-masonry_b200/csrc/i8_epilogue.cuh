@@ -21,7 +21,7 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
 
 // silu(gate) * up = gate / (1 + exp(-gate)) * up.  ex2.approx and rcp.approx are within 2^-22 relative, the
 // rounded exponent argument adds |gate| 2^-24: far below the 2^-8 of the bf16 that follows.  For gate below
-// -88 the exponential overflows to infinity and the result is -0.
+// -87 the reciprocal would be subnormal, and the result is -0.
 __device__ __forceinline__ float silu_mul(float gate, float up) {
   float e, r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(gate * -1.4426950408889634f));

@@ -202,22 +202,23 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
       if (row >= 0) p.slot_of_row[row] = s;
     }
   }
-  // Rows that no slot names: the padding of every group, and everything behind the last one.
-  const int threads = ctas * blockDim.x;
-  const int me = rank * blockDim.x + threadIdx.x;
+  // Rows that no slot names: the padding of every group, and everything behind the last one.  Unsigned, since
+  // a step past the last row may leave 31 bits.
+  const unsigned threads = ctas * blockDim.x;
+  const unsigned me = rank * blockDim.x + threadIdx.x;
   if (p.align > 1) {
     for (int e = me >> 5; e < G; e += threads >> 5) {
-      const int end = e + 1 < G ? total[e + 1] : used;
-      for (int r = total[e] + count[e] + lane; r < end; r += 32) p.slot_of_row[r] = -1;
+      const unsigned end = e + 1 < G ? total[e + 1] : used;
+      for (unsigned r = total[e] + count[e] + lane; r < end; r += 32) p.slot_of_row[r] = -1;
     }
   }
-  for (int r = used + me; r < p.cap; r += threads) p.slot_of_row[r] = -1;
+  for (unsigned r = used + me; r < static_cast<unsigned>(p.cap); r += threads) p.slot_of_row[r] = -1;
   if (p.mtile_group != nullptr) {
     for (int e = me >> 5; e < G; e += threads >> 5) {
       const int end = e + 1 < G ? total[e + 1] : used;
       for (int t = total[e] / 256 + lane; t < end / 256; t += 32) p.mtile_group[t] = e;
     }
-    for (int t = used / 256 + me; t < p.cap / 256; t += threads) p.mtile_group[t] = G - 1;
+    for (int t = used / 256 + static_cast<int>(me); t < p.cap / 256; t += threads) p.mtile_group[t] = G - 1;
   }
 }
 

@@ -50,7 +50,7 @@ int check_quantize(const void* src, int64_t ld_src, const void* codes, int64_t l
                    int64_t K) {
   if (rows != 0 && (src == nullptr || codes == nullptr || scales == nullptr))
     return set_error(SMB_ERR_INVALID, "i8 quantize: null pointer");
-  if (rows < 0 || rows > 0x7FFFFFFFLL || K <= 0 || K > 0x7FFFFFFFLL)
+  if (rows < 0 || rows > 0x7FFFFFFFLL || K <= 0 || K > (1LL << 30))   // 32-bit steps through a row
     return set_error(SMB_ERR_INVALID, "i8 quantize: bad extents (rows=%lld K=%lld)", static_cast<long long>(rows),
                      static_cast<long long>(K));
   if (ld_src < K || ld_bytes < K) return set_error(SMB_ERR_INVALID, "i8 quantize: pitch smaller than K");

@@ -176,3 +176,14 @@ def test_row_copy_refusals(smb):
     _refused(smb, lib.smb_moe_combine_backward_device(P, 64, P, 64, P, P, 4, 2, 64, 8, P, 60, P, None), "pitch")
     _refused(smb, lib.smb_moe_route_backward_device(P, 0, 64, None, P, 4, 64, 2, 0, 1.0, P, 64, None), "null")
     _refused(smb, lib.smb_moe_route_backward_device(P, 0, 64, P, P, 4, 64, 2, 0, 1.0, P, 63, None), "pitch")
+
+
+def test_extents_that_leave_31_bits_are_refused(smb):
+    lib = smb.capi.lib()
+    inv, uns = smb.capi.SMB_ERR_INVALID, smb.capi.SMB_ERR_UNSUPPORTED
+    big = (1 << 30) + 1
+    h = C.c_void_p()
+    assert lib.smb_i8_plan_create(C.byref(h), P, P, P, P, P, big, 8, 16, 16, 16, 8, 0) == uns
+    assert lib.smb_i8_plan_create(C.byref(h), P, P, P, P, P, 8, big, 16, 16, 16, big + 7, 0) == uns
+    assert lib.smb_quantize_i8_device(P, big, P, big, P, 1, big, None) == inv
+    assert lib.smb_quantize_i8_bf16_device(P, big, P, big, P, 1, big, None) == inv
