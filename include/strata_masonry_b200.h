@@ -551,6 +551,20 @@ int smb_moe_combine_backward_device(const uint16_t* grad_y, int64_t ld_grad_y, c
                                     uint16_t* grad_rows, int64_t ld_grad_rows, float* grad_weights,
                                     void* stream);
 
+/* The stream-ordered calls above with their arguments as `count` 64-bit words in the order of the prototype
+ * (pointers, integers and flags by value, `scale` as the bits of a double), for bindings that pay for every
+ * argument.  A value that does not fit its parameter is refused. */
+#define SMB_CALL_QUANTIZE_I8 0
+#define SMB_CALL_QUANTIZE_I8_BF16 1
+#define SMB_CALL_MOE_ROUTE 2
+#define SMB_CALL_MOE_ROUTE_BACKWARD 3
+#define SMB_CALL_MOE_DISPATCH 4
+#define SMB_CALL_MOE_GATHER_BF16 5
+#define SMB_CALL_MOE_GATHER_I8 6
+#define SMB_CALL_MOE_COMBINE 7
+#define SMB_CALL_MOE_COMBINE_BACKWARD 8
+int smb_call_words(int call, const void* words, int count);
+
 #define SMB_FLAG_NONE 0u
 #define SMB_FLAG_FORCE_PLAIN_STORE 1u /* use the non-TMA epilogue even when D is aligned */
 #define SMB_FLAG_TILE_N_128 2u        /* force 256 x 128 tiles */

@@ -31,7 +31,7 @@ COMMON = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-
 
 LIB_SOURCES = ["runtime.cu", "fills.cu", "gemm_bf16.cu", "gemm_bf16_streamk.cu", "api_bf16.cu", "gemm_nvfp4.cu",
                "gemm_nvfp4_arun.cu", "gemm_nvfp4_decode.cu", "api_nvfp4.cu", "peer.cu", "gather.cu", "selftest.cu", "quant_i8.cu",
-               "gemm_i8.cu", "gemm_i8_decode.cu", "api_i8.cu", "moe_route.cu", "moe_rows.cu"]
+               "gemm_i8.cu", "gemm_i8_decode.cu", "api_i8.cu", "moe_route.cu", "moe_rows.cu", "api_words.cu"]
 DRIVERS = {"kernel_sm100a_dense_gemm_bf16": "driver_bf16.cu",
            "kernel_sm100a_dense_gemm_nvfp4": "driver_nvfp4.cu"}
 

@@ -50,6 +50,16 @@ ROUTE_SIGMOID = 1
 ROUTE_RENORM = 2
 ROUTE_GROUP_TOP2 = 4
 
+CALL_QUANTIZE_I8 = 0
+CALL_QUANTIZE_I8_BF16 = 1
+CALL_MOE_ROUTE = 2
+CALL_MOE_ROUTE_BACKWARD = 3
+CALL_MOE_DISPATCH = 4
+CALL_MOE_GATHER_BF16 = 5
+CALL_MOE_GATHER_I8 = 6
+CALL_MOE_COMBINE = 7
+CALL_MOE_COMBINE_BACKWARD = 8
+
 _vp = C.c_void_p
 _i = C.c_int
 _i64 = C.c_int64
@@ -169,6 +179,7 @@ DECLARED = [
     ("smb_moe_combine_device", _i, [_vp, _i64, _vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp]),
     ("smb_moe_combine_backward_device", _i,
      [_vp, _i64, _vp, _i64, _vp, _vp, _i64, _i, _i, _i64, _vp, _i64, _vp, _vp]),
+    ("smb_call_words", _i, [_i, C.c_char_p, _i]),
 ]
 
 PEER_HANDLE_BYTES = 64
@@ -185,11 +196,12 @@ class SmbError(RuntimeError):
 
 
 _lib = None
+_call_words = None
 
 
 def lib() -> C.CDLL:
     """Load the library once and attach prototypes."""
-    global _lib
+    global _lib, _call_words
     if _lib is not None:
         return _lib
     if not LIB_PATH.exists():
@@ -201,6 +213,9 @@ def lib() -> C.CDLL:
         fn = getattr(handle, name)
         fn.restype = restype
         fn.argtypes = argtypes
+    # A function object of its own without a prototype: ctypes then passes small integers and strings as they
+    # are, which costs a third of converting them.
+    _call_words = handle["smb_call_words"]
     _lib = handle
     return handle
 
@@ -210,5 +225,14 @@ def last_error() -> str:
 
 
 def check(code: int) -> None:
+    if code != SMB_OK:
+        raise SmbError(code, last_error())
+
+
+def call_words(call: int, words: bytes, count: int) -> None:
+    """One of the stream-ordered calls (CALL_*) with its arguments packed as 64-bit words."""
+    if _call_words is None:
+        lib()
+    code = _call_words(call, words, count)
     if code != SMB_OK:
         raise SmbError(code, last_error())

@@ -8,6 +8,7 @@ timing loops use.  Nothing in here computes on the CPU.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -24,6 +25,16 @@ def _ptr(x) -> int:
     if isinstance(x, np.ndarray):
         return int(x.ctypes.data)
     raise TypeError(f"cannot take the address of {type(x)!r}")
+
+
+def _addr(x) -> int:
+    """_ptr, the common kinds of device buffers first."""
+    if x is None:
+        return 0
+    try:
+        return x.data_ptr()
+    except AttributeError:
+        return _ptr(x)
 
 
 def _stream_ptr(stream) -> int:
@@ -394,6 +405,9 @@ class Fp4HostContext:
 
 
 # ------------------------------------------------------------------------------- int8
+_QUANTIZE_I8 = struct.Struct("@8q").pack
+
+
 def quantize_i8_host(src: np.ndarray):
     """FP32 [rows, K] -> (int8 codes [rows, K], fp32 scales [rows]), one scale per row."""
     src = np.ascontiguousarray(src, dtype=np.float32)
@@ -407,17 +421,17 @@ def quantize_i8_host(src: np.ndarray):
 def quantize_i8_device(src, codes, scales, rows: int, k: int, ld_src: int | None = None, ld_bytes: int | None = None,
                        stream=None) -> None:
     """FP32 rows on the device -> int8 codes and one scale per row."""
-    capi.check(capi.lib().smb_quantize_i8_device(
-        _ptr(src), k if ld_src is None else ld_src, _ptr(codes), k if ld_bytes is None else ld_bytes, _ptr(scales),
-        rows, k, _stream_ptr(stream)))
+    capi.call_words(capi.CALL_QUANTIZE_I8, _QUANTIZE_I8(
+        _addr(src), k if ld_src is None else ld_src, _addr(codes), k if ld_bytes is None else ld_bytes, _addr(scales),
+        rows, k, _stream_ptr(stream)), 8)
 
 
 def quantize_i8_bf16_device(src, codes, scales, rows: int, k: int, ld_src: int | None = None,
                             ld_bytes: int | None = None, stream=None) -> None:
     """BF16 rows on the device -> int8 codes and one scale per row."""
-    capi.check(capi.lib().smb_quantize_i8_bf16_device(
-        _ptr(src), k if ld_src is None else ld_src, _ptr(codes), k if ld_bytes is None else ld_bytes, _ptr(scales),
-        rows, k, _stream_ptr(stream)))
+    capi.call_words(capi.CALL_QUANTIZE_I8_BF16, _QUANTIZE_I8(
+        _addr(src), k if ld_src is None else ld_src, _addr(codes), k if ld_bytes is None else ld_bytes, _addr(scales),
+        rows, k, _stream_ptr(stream)), 8)
 
 
 def dense_gemm_i8_host(a: np.ndarray, sa: np.ndarray, b: np.ndarray, sb: np.ndarray) -> np.ndarray:

@@ -187,3 +187,62 @@ def test_extents_that_leave_31_bits_are_refused(smb):
     assert lib.smb_i8_plan_create(C.byref(h), P, P, P, P, P, 8, big, 16, 16, 16, big + 7, 0) == uns
     assert lib.smb_quantize_i8_device(P, big, P, big, P, 1, big, None) == inv
     assert lib.smb_quantize_i8_bf16_device(P, big, P, big, P, 1, big, None) == inv
+
+
+def test_calls_by_words_take_the_same_arguments(smb):
+    """Every argument lands in its own parameter: one bad value at a time comes back as that refusal."""
+    moe, gemm, err = smb.moe, smb.gemm, smb.SmbError
+    p, odd = P.value, ODD.value
+    route = dict(logits=p, ids=p, weights=p, tokens=8, experts=64, top_k=4, n_groups=8, top_groups=4)
+    moe.route_device(**dict(route, tokens=0))
+    for change, text in [(dict(logits=odd), "logits are not aligned"), (dict(dtype=2), "dtype 2"), (dict(ld=63), "pitch"),
+                         (dict(bias=odd), "4-byte"), (dict(tokens=-1), "negative"), (dict(tokens=1 << 40), "does not fit"),
+                         (dict(experts=513), "513 experts"), (dict(top_k=33), "top_k=33"), (dict(n_groups=7), "7 groups"),
+                         (dict(top_groups=9), "top_groups=9"), (dict(flags=64), "0x40"), (dict(flags=-1), "does not fit"),
+                         (dict(ids=None), "null output"), (dict(weights=odd), "4-byte")]:
+        with pytest.raises(err, match=text):
+            moe.route_device(**dict(route, **change))
+    grad = dict(logits=p, ids=p, grad_weights=p, grad_logits=p, tokens=8, experts=64, top_k=4)
+    moe.route_backward_device(**dict(grad, tokens=0))
+    for change, text in [(dict(ids=odd), "ids and gradients"), (dict(grad_weights=None), "null"), (dict(grad_logits=odd), "gradient is not"),
+                         (dict(ld_grad=63), "gradient pitch"), (dict(ld=63), "pitch"), (dict(top_k=0), "top_k=0"), (dict(flags=8), "0x8")]:
+        with pytest.raises(err, match=text):
+            moe.route_backward_device(**dict(grad, **change))
+    sort = dict(ids=p, offsets=p, row_of_slot=p, slot_of_row=p, tokens=8, top_k=2, groups=4, max_rows=16)
+    for change, text in [(dict(offsets=None), "null"), (dict(slot_of_row=odd), "4-byte"), (dict(tokens=-1), "tokens=-1"),
+                         (dict(top_k=33), "top_k=33"), (dict(groups=1025), "1025 groups"), (dict(max_rows=15), "room for 15 rows"),
+                         (dict(align=0), "alignment 0"), (dict(mtile_group=p), "tile map")]:
+        with pytest.raises(err, match=text):
+            moe.dispatch_device(**dict(sort, **change))
+    for call, args in [(moe.gather_bf16_device, dict(x=p, row_of_slot=p, out=p)),
+                       (moe.gather_i8_device, dict(x=p, row_of_slot=p, codes=p, scales=p)),
+                       (moe.combine_device, dict(rows=p, row_of_slot=p, weights=p, y=p)),
+                       (moe.combine_backward_device, dict(grad_y=p, rows=p, row_of_slot=p, weights=p, grad_rows=p, grad_weights=p))]:
+        dims = dict(tokens=4, top_k=2, width=64, max_rows=8)
+        call(**args, **dict(dims, tokens=0))
+        pitches = [n for n in call.__code__.co_varnames if n.startswith("ld_")]
+        assert pitches
+        for change, text in [(dict(tokens=-1), "token count"), (dict(top_k=33), "top_k=33"), (dict(width=0), "width 0"),
+                             (dict(max_rows=0), "capacity")] + [({n: 63}, "pitch") for n in pitches]:
+            with pytest.raises(err, match=text):
+                call(**args, **dict(dims, **change))
+        for n in args:
+            if args[n] == p and n not in ("codes",):
+                with pytest.raises(err, match="aligned"):
+                    call(**dict(args, **{n: odd}), **dims)
+    for call in (gemm.quantize_i8_device, gemm.quantize_i8_bf16_device):
+        call(p, p, p, 0, 64)
+        for args, kw, text in [((None, p, p, 2, 64), {}, "null"), ((p, p, p, -1, 64), {}, "rows=-1"), ((p, p, p, 2, 0), {}, "K=0"),
+                               ((p, p, p, 2, 64), dict(ld_src=63), "pitch"), ((p, p, p, 2, 64), dict(ld_bytes=63), "pitch"),
+                               ((odd, p, p, 2, 64), {}, "aligned"), ((p, p, odd, 2, 64), {}, "aligned")]:
+            with pytest.raises(err, match=text):
+                call(*args, **kw)
+
+
+def test_calls_by_words_refusals(smb):
+    words = smb.capi.lib().smb_call_words
+    _refused(smb, words(99, b"\0" * 64, 8), "unknown call 99")
+    _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, b"\0" * 56, 7), "7 words for 8 arguments")
+    _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, None, 8), "no words")
+    _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, b"\0" * 120, 15), "no words")
+    _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, b"\0" * 8, -1), "no words")
