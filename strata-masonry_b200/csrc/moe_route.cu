@@ -113,8 +113,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return y;
 }
 
-// Logits as this file uses them: closed experts are -inf, +inf is the largest finite value.
-__device__ __forceinline__ float clean_logit(float l) { return fminf(fmaxf(l, -INFINITY), FLT_MAX); }
+// Logits as this file uses them: closed experts are -inf, +inf is the largest finite value, and zero has no
+// sign (keys would put +0 above -0).
+__device__ __forceinline__ float clean_logit(float l) { return fminf(fmaxf(l, -INFINITY), FLT_MAX) + 0.0f; }
 
 template <bool kBf16>
 __device__ __forceinline__ float load_logit(const void* row, int e) {
@@ -411,7 +412,10 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
   float l[V];
   load_run<V, kBf16>(row, e0, valid ? p.experts : 0, p.wide, l);
   float top = 0.0f;
-  if (!sigmoid) {
+  if (sigmoid) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] += 0.0f;   // as clean_logit does
+  } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) l[i] = clean_logit(l[i]);
     top = l[0];

@@ -169,6 +169,25 @@ def test_route_extreme_logits(smb, cuda_device):
     np.testing.assert_allclose(w.cpu().numpy(), [[1, np.exp(-50)]], rtol=2 ** -17)
 
 
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("experts", [16, 64, 256, 512])
+def test_route_zeros_of_either_sign_tie(smb, cuda_device, sigmoid, bf16, experts):
+    """Logits masked by a product are zeros of both signs; they are equal, so the lowest index comes first."""
+    torch = _torch()
+    c = smb.capi
+    rng = np.random.default_rng(experts)
+    l = np.where(rng.random((40, experts)) < 0.5, np.float32(0.0), np.float32(-0.0))
+    l[1:20, 3::7] = 1.0                       # some above, the rest of the choices among the zeros
+    l[5:30, 5::9] = -1.0
+    flags = (c.ROUTE_SIGMOID if sigmoid else 0) | c.ROUTE_RENORM
+    for groups in (1, 8):
+        _, ids, _ = _route(smb, torch, l, c.DTYPE_BF16 if bf16 else c.DTYPE_F32, 8, n_groups=groups, top_groups=max(1, groups // 2),
+                           flags=flags)
+        want, _ = _route_plain(l.astype(np.float64), None, 8, groups, max(1, groups // 2), sigmoid, True, False, 1.0)
+        np.testing.assert_array_equal(ids.cpu().numpy(), want)
+
+
 # ------------------------------------------------------------------ routing, gradient
 def _weights_of(l, ids, sigmoid, renorm, scale):
     """Weights as a function of the logits for fixed ids (float64), for differences."""
