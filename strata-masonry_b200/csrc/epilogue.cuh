@@ -83,6 +83,69 @@ __device__ __forceinline__ void release_columns(uint32_t release_bar, int lane) 
   if (lane == 0) mbar_arrive_cluster_no_release(release_bar);
 }
 
+// A staged 32 x 64 box to a D of any alignment: consecutive lanes write consecutive columns of a row, pairs of
+// them where D takes 4-byte stores.  Bound by instructions, so whole boxes take a straight path (two or three
+// instructions a store; with bounds and addresses for each it was twelve).
+__device__ __forceinline__ void store_box_plain(uint32_t sbuf, const StoreTarget& out, int row0, int gcol0, int lane) {
+  const int rows = min(out.M, out.row_end) - row0;
+  if (rows <= 0) return;
+  uint16_t* dst = out.d_ptr + static_cast<size_t>(row0) * out.ldd + gcol0;
+  auto at = [&](int r, int c) { return sbuf + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | ((c & 7) << 1)); };
+  if (rows >= 32 && gcol0 + kStoreCols <= out.N) {
+    const bool pairs = ((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(out.ldd) * 2) & 3) == 0;
+    if (pairs) {
+      uint32_t* p = reinterpret_cast<uint32_t*>(dst) + lane;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint32_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ld_shared_u32(at(i, 2 * lane) + r0 * 128);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          *p = v[i];
+          p = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(p) + out.ldd);
+        }
+      }
+    } else {
+      uint16_t* p = dst + lane;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 32; r0 += 8) {
+        uint16_t v[8][2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[i][h]) : "r"(at(i, h * 32 + lane) + r0 * 128) : "memory");
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[0] = v[i][0];
+          p[32] = v[i][1];
+          p += out.ldd;
+        }
+      }
+    }
+    return;
+  }
+  const bool in0 = gcol0 + lane < out.N, in1 = gcol0 + 32 + lane < out.N;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32 && r0 < rows; r0 += 8) {
+    uint16_t v[8][2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[i][h]) : "r"(at(i, h * 32 + lane) + r0 * 128) : "memory");
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (in0 && r0 + i < rows) dst[lane] = v[i][0];
+      if (in1 && r0 + i < rows) dst[32 + lane] = v[i][1];
+      dst += out.ldd;
+    }
+  }
+}
+
 // Phase 2 alone: kOutCols packed columns to D rows [row0, row0 + 32), columns [col0, col0 + kOutCols),
 // in 64-column boxes through the warp's staging buffer.
 template <int kOutCols, bool kTmaStore>
@@ -158,21 +221,8 @@ __device__ __forceinline__ void store_columns(const uint32_t (&packed)[kOutCols 
         }
       }
     } else {
-      // Read the staged box back so that consecutive lanes write consecutive columns of a row.
       __syncwarp();
-      for (int r = 0; r < 32; ++r) {
-        const int grow = row0 + r;
-        if (grow >= out.M || grow >= out.row_end) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int cc = h * 32 + lane;
-          const int gcol = gcol0 + cc;
-          const uint32_t src = sbuf + r * 128 + ((((cc >> 3) ^ (r & 7)) << 4) | ((cc & 7) << 1));
-          uint16_t val;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(val) : "r"(src) : "memory");
-          if (gcol < out.N) out.d_ptr[static_cast<size_t>(grow) * out.ldd + gcol] = val;
-        }
-      }
+      store_box_plain(sbuf, out, row0, gcol0, lane);
       __syncwarp();
     }
   }
