@@ -44,6 +44,7 @@ struct DispatchParams {
   int groups, align;
   int cap;             // rows of the sorted buffer
   int per_warp;        // slots per warp, a multiple of 32
+  int sorters;         // warps of a CTA that own slots; the rest only help with groups and rows
   int* offsets;
   int* row_of_slot;
   int* slot_of_row;
@@ -53,7 +54,7 @@ struct DispatchParams {
 // One cluster sorts everything: warp w of the cluster owns the slots [w * per_warp, + per_warp), so
 // "earlier slots" means earlier lanes, earlier chunks, earlier warps, earlier CTAs, and the counts of the
 // CTAs meet through distributed shared memory instead of a second launch.
-//   shared: hist[warps][groups] | total[groups] | start[groups] | count[groups]
+//   shared: hist[sorters][groups] | total[groups] | start[groups] | count[groups]
 // Bound by latency: the ids of a warp are fetched together (8 x 32 at a time) and stay in registers
 // between the count and the placement where they fit.  128 slots of 256 groups 2.3 us, 4096 of 64 4.3 us; 65536
 // slots 9.8 us on the eight SMs of a cluster, where the copies that follow take 190.
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   extern __shared__ int sm[];
   __shared__ int warp_sums[32];
   griddep_launch_dependents();
-  const int warps = blockDim.x >> 5;
+  const int all_warps = blockDim.x >> 5, warps = p.sorters;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ctas = kCluster ? static_cast<int>(cluster_nctarank()) : 1;
   const int rank = kCluster ? static_cast<int>(cluster_ctarank()) : 0;
@@ -88,11 +89,12 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   int* start = total + G;
   int* count = start + G;
 
-  const long long first = static_cast<long long>(rank * warps + warp) * p.per_warp;
+  const long long first = warp < warps ? static_cast<long long>(rank * warps + warp) * p.per_warp : p.n;
   const int lo = static_cast<int>(first < p.n ? first : p.n);
   const int hi = static_cast<int>(first + p.per_warp < p.n ? first + p.per_warp : p.n);
-  int* mine = hist + warp * G;
-  for (int e = lane; e < G; e += 32) mine[e] = 0;
+  int* mine = hist + warp * G;   // of sorters
+  if (warp < warps)
+    for (int e = lane; e < G; e += 32) mine[e] = 0;
   griddep_wait();
   int held[kHeldIds];
 #pragma unroll
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   if (lane == 31) warp_sums[warp] = inclusive;
   if (kCluster) cluster_sync_all();   // nobody's totals are read by another CTA after this
   else __syncthreads();
-  const int others = lane < warps ? warp_sums[lane] : 0;
+  const int others = lane < all_warps ? warp_sums[lane] : 0;
   int base = __reduce_add_sync(kFull, lane < warp ? others : 0) + inclusive - sum;
   const int used = __reduce_add_sync(kFull, others);
   const int id_bits = 32 - __clz(G);   // G < 2^bits, so the low bits of -1 are no id either
@@ -225,29 +227,36 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
 // --------------------------------------------------------------------------- gather
 constexpr int kCta = 256;
 
-template <bool kAligned>
+// Rows are read and written in words of 16, 4 or 2 bytes, the widest that bases, pitches and width allow,
+// consecutive lanes on consecutive words; a thread has kWords of them in flight.
+template <class W>
+struct Words {
+  static constexpr int kElems = sizeof(W) / 2;
+  static constexpr int kWords = sizeof(W) == 16 ? 1 : 4;
+};
+
+template <class W>
 __global__ void __launch_bounds__(kCta) gather_bf16_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int top_k,
                                                            int width, int max_rows, uint16_t* out, int64_t ld_out) {
+  constexpr int kE = Words<W>::kElems, kN = Words<W>::kWords;
   griddep_launch_dependents();
   griddep_wait();
   const int64_t t = blockIdx.x;
   const int* rows = row_of_slot + t * top_k;
-  const uint16_t* src = x + t * ld_x;
-  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
-  if (c0 >= width) return;
-  if (kAligned && c0 + 8 <= width) {
-    const uint4 v = *reinterpret_cast<const uint4*>(src + c0);
-    for (int j = 0; j < top_k; ++j) {
-      const int r = rows[j];
-      if (r >= 0 && r < max_rows) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(r) * ld_out + c0) = v;
-    }
-    return;
-  }
-  const int end = min(c0 + 8, width);
+  const W* src = reinterpret_cast<const W*>(x + t * ld_x);
+  const int words = width / kE;
+  const int c0 = blockIdx.y * kN * blockDim.x + threadIdx.x;
+  W v[kN];
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+    if (c0 + i * blockDim.x < words) v[i] = src[c0 + i * blockDim.x];
   for (int j = 0; j < top_k; ++j) {
     const int r = rows[j];
     if (r < 0 || r >= max_rows) continue;
-    for (int c = c0; c < end; ++c) out[static_cast<int64_t>(r) * ld_out + c] = src[c];
+    W* dst = reinterpret_cast<W*>(out + static_cast<int64_t>(r) * ld_out);
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (c0 + i * blockDim.x < words) dst[c0 + i * blockDim.x] = v[i];
   }
 }
 
@@ -267,7 +276,7 @@ gather_i8_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int64_
   // its stores.
   int* rows = rows_all[kWarp ? threadIdx.x >> 5 : 0];
   if (tid < top_k) rows[tid] = row_of_slot[t * top_k + tid];
-  const float scale = qi8::quantize_row<true, kWarp, kAligned>(
+  const float scale = qi8::quantize_row<true, kWarp, kAligned, true>(
       x + t * ld_x, width, tid, threads, red,
       [&](int k, uint2 c) {
         for (int j = 0; j < top_k; ++j) {
@@ -290,25 +299,29 @@ gather_i8_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int64_
 // --------------------------------------------------------------------------- combine
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ float bf16_one(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
-__device__ __forceinline__ uint16_t to_bf16(float v) {
-  return static_cast<uint16_t>(pack_bf16x2(__float_as_uint(v), 0u) & 0xFFFFu);
-}
+
+// A word of bf16 as 32-bit pairs (a single element as the low half of one).
+__device__ __forceinline__ uint32_t pair_of(const uint4& q, int i) { return i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w)); }
+__device__ __forceinline__ uint32_t pair_of(uint32_t q, int) { return q; }
+__device__ __forceinline__ uint32_t pair_of(uint16_t q, int) { return q; }
+__device__ __forceinline__ void set_word(uint4& q, const uint32_t* p) { q = make_uint4(p[0], p[1], p[2], p[3]); }
+__device__ __forceinline__ void set_word(uint32_t& q, const uint32_t* p) { q = p[0]; }
+__device__ __forceinline__ void set_word(uint16_t& q, const uint32_t* p) { q = static_cast<uint16_t>(p[0] & 0xFFFFu); }
 
 // fp32 sum in slot order, one rounding to bf16.
-template <bool kAligned>
+template <class W>
 __global__ void __launch_bounds__(kCta) combine_kernel(const uint16_t* rows_in, int64_t ld_rows, const int* row_of_slot,
                                                        const float* weights, int top_k, int width, int max_rows, uint16_t* y,
                                                        int64_t ld_y) {
+  constexpr int kE = Words<W>::kElems, kN = Words<W>::kWords, kPairs = (kE + 1) / 2;
   griddep_launch_dependents();
   griddep_wait();
   const int64_t t = blockIdx.x;
   const int* rows = row_of_slot + t * top_k;
-  const int c0 = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
-  if (c0 >= width) return;
-  float acc[8] = {};
-  const int n = min(8, width - c0);
-  const bool whole = kAligned && n == 8;
+  const int words = width / kE;
+  const int c0 = blockIdx.y * kN * blockDim.x + threadIdx.x;
+  if (c0 >= words) return;
+  float acc[kN][2 * kPairs] = {};
   const float* w_row = weights != nullptr ? weights + t * top_k : nullptr;
   // Eight slots at a time: their rows, then all their loads, are in flight together.
   for (int j0 = 0; j0 < top_k; j0 += 8) {
@@ -320,54 +333,44 @@ __global__ void __launch_bounds__(kCta) combine_kernel(const uint16_t* rows_in, 
       w[i] = w_row != nullptr && j0 + i < top_k ? w_row[j0 + i] : 1.0f;
       if (r[i] >= max_rows) r[i] = -1;
     }
-    if (whole) {
-      uint4 q[8];
+    W q[8][kN];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r[i] >= 0) q[i] = *reinterpret_cast<const uint4*>(rows_in + static_cast<int64_t>(r[i]) * ld_rows + c0);
+    for (int i = 0; i < 8; ++i) {
+      const W* src = reinterpret_cast<const W*>(rows_in + static_cast<int64_t>(r[i]) * ld_rows);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r[i] < 0) continue;
-        const uint32_t v[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+      for (int n = 0; n < kN; ++n)
+        if (r[i] >= 0 && c0 + n * blockDim.x < words) q[i][n] = src[c0 + n * blockDim.x];
+    }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          acc[2 * k] = fmaf(w[i], bf16_lo(v[k]), acc[2 * k]);
-          acc[2 * k + 1] = fmaf(w[i], bf16_hi(v[k]), acc[2 * k + 1]);
+    for (int i = 0; i < 8; ++i) {
+      if (r[i] < 0) continue;
+#pragma unroll
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) {
+          acc[n][2 * k] = fmaf(w[i], bf16_lo(pair_of(q[i][n], k)), acc[n][2 * k]);
+          if (kE > 1) acc[n][2 * k + 1] = fmaf(w[i], bf16_hi(pair_of(q[i][n], k)), acc[n][2 * k + 1]);
         }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r[i] < 0) continue;
-        const uint16_t* src = rows_in + static_cast<int64_t>(r[i]) * ld_rows + c0;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (k < n) acc[k] = fmaf(w[i], bf16_one(src[k]), acc[k]);
-      }
     }
   }
-  uint16_t* dst = y + t * ld_y + c0;
-  if (whole) {
-    uint4 q;
-    q.x = pack_bf16x2(__float_as_uint(acc[0]), __float_as_uint(acc[1]));
-    q.y = pack_bf16x2(__float_as_uint(acc[2]), __float_as_uint(acc[3]));
-    q.z = pack_bf16x2(__float_as_uint(acc[4]), __float_as_uint(acc[5]));
-    q.w = pack_bf16x2(__float_as_uint(acc[6]), __float_as_uint(acc[7]));
-    *reinterpret_cast<uint4*>(dst) = q;
-  } else {
+  W* dst = reinterpret_cast<W*>(y + t * ld_y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < n) dst[i] = to_bf16(acc[i]);
+  for (int n = 0; n < kN; ++n) {
+    uint32_t o[kPairs];
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) o[k] = pack_bf16x2(__float_as_uint(acc[n][2 * k]), __float_as_uint(acc[n][2 * k + 1]));
+    if (c0 + n * blockDim.x < words) set_word(dst[c0 + n * blockDim.x], o);
   }
 }
 
 // A warp per slot: its row's gradient w * dy and its weight's gradient <dy, row>.  The warps of a token
 // are neighbours, so dy comes from L1 after the first of them.
-template <bool kAligned>
+template <class W>
 __global__ void __launch_bounds__(kCta) combine_grad_kernel(const uint16_t* grad_y, int64_t ld_gy, const uint16_t* rows_in,
                                                             int64_t ld_rows, const int* row_of_slot, const float* weights,
                                                             int64_t slots, int top_k, int width, int max_rows,
                                                             uint16_t* grad_rows, int64_t ld_gr, float* grad_weights) {
+  constexpr int kE = Words<W>::kElems, kN = kE == 1 ? 8 : Words<W>::kWords, kPairs = (kE + 1) / 2;
   griddep_launch_dependents();
   griddep_wait();
   const int lane = threadIdx.x & 31;
@@ -379,33 +382,34 @@ __global__ void __launch_bounds__(kCta) combine_grad_kernel(const uint16_t* grad
     return;
   }
   const float w = weights != nullptr ? weights[s] : 1.0f;
-  const uint16_t* gy = grad_y + s / top_k * ld_gy;
-  const uint16_t* in = rows_in != nullptr ? rows_in + static_cast<int64_t>(r) * ld_rows : nullptr;
-  uint16_t* out = grad_rows + static_cast<int64_t>(r) * ld_gr;
+  const W* gy = reinterpret_cast<const W*>(grad_y + s / top_k * ld_gy);
+  const W* in = grad_weights != nullptr ? reinterpret_cast<const W*>(rows_in + static_cast<int64_t>(r) * ld_rows) : nullptr;
+  W* out = reinterpret_cast<W*>(grad_rows + static_cast<int64_t>(r) * ld_gr);
   float dot = 0.0f;
-  const int whole = kAligned ? width / 8 * 8 : 0;
-  for (int c = lane * 8; c < whole; c += 256) {
-    const uint4 g4 = *reinterpret_cast<const uint4*>(gy + c);
-    const uint32_t g[4] = {g4.x, g4.y, g4.z, g4.w};
-    if (grad_weights != nullptr) {
-      const uint4 v4 = *reinterpret_cast<const uint4*>(in + c);
-      const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
+  const int words = width / kE;
+  for (int c = lane; c < words; c += 32 * kN) {
+    W g[kN], v[kN];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        dot = fmaf(bf16_lo(g[i]), bf16_lo(v[i]), dot);
-        dot = fmaf(bf16_hi(g[i]), bf16_hi(v[i]), dot);
-      }
+    for (int n = 0; n < kN; ++n) {
+      if (c + 32 * n >= words) continue;
+      g[n] = gy[c + 32 * n];
+      if (in != nullptr) v[n] = in[c + 32 * n];
     }
-    uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o[i] = pack_bf16x2(__float_as_uint(w * bf16_lo(g[i])), __float_as_uint(w * bf16_hi(g[i])));
-    *reinterpret_cast<uint4*>(out + c) = make_uint4(o[0], o[1], o[2], o[3]);
-  }
-  for (int c = whole + lane; c < width; c += 32) {
-    const float g = bf16_one(gy[c]);
-    if (grad_weights != nullptr) dot = fmaf(g, bf16_one(in[c]), dot);
-    out[c] = to_bf16(w * g);
+    for (int n = 0; n < kN; ++n) {
+      if (c + 32 * n >= words) continue;
+      uint32_t o[kPairs];
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) {
+        const float lo = bf16_lo(pair_of(g[n], k)), hi = bf16_hi(pair_of(g[n], k));   // hi of a single element: 0
+        if (in != nullptr) {
+          dot = fmaf(lo, bf16_lo(pair_of(v[n], k)), dot);
+          if (kE > 1) dot = fmaf(hi, bf16_hi(pair_of(v[n], k)), dot);
+        }
+        o[k] = pack_bf16x2(__float_as_uint(w * lo), __float_as_uint(w * hi));
+      }
+      set_word(out[c + 32 * n], o);
+    }
   }
   if (grad_weights != nullptr) {
 #pragma unroll
@@ -415,6 +419,10 @@ __global__ void __launch_bounds__(kCta) combine_grad_kernel(const uint16_t* grad
 }
 
 bool aligned16(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
+// Whether rows of 2-byte elements consist of words of n bytes.
+bool rows_take(int n, const void* p, int64_t ld, int width) {
+  return reinterpret_cast<uintptr_t>(p) % n == 0 && ld * 2 % n == 0 && static_cast<int64_t>(width) * 2 % n == 0;
+}
 bool aligned_to(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int finish(cudaError_t e, const char* what) {
@@ -435,13 +443,49 @@ int check_rows(const char* what, const void* row_of_slot, int64_t tokens, int to
   return SMB_OK;
 }
 
-// Threads for a row in vectors of eight: whole warps, at most a CTA; the rest goes to the grid's y.
+// Threads for a row in words: whole warps, at most 128; the rest goes to the grid's y.
+template <class W>
 void row_grid(int64_t tokens, int width, dim3* grid, dim3* block) {
-  const int vecs = (width + 7) / 8;
-  int threads = (vecs + 31) / 32 * 32;
+  const int words = width / Words<W>::kElems;
+  int threads = (words + Words<W>::kWords * 32 - 1) / (Words<W>::kWords * 32) * 32;
   if (threads > 128) threads = 128;
+  const int per_cta = threads * Words<W>::kWords;
   *block = dim3(static_cast<unsigned>(threads), 1, 1);
-  *grid = dim3(static_cast<unsigned>(tokens), static_cast<unsigned>((vecs + threads - 1) / threads), 1);
+  *grid = dim3(static_cast<unsigned>(tokens), static_cast<unsigned>((words + per_cta - 1) / per_cta), 1);
+}
+
+template <class W>
+int launch_gather(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens, int top_k, int width, int max_rows,
+                  uint16_t* out, int64_t ld_out, void* stream) {
+  dim3 grid, block;
+  row_grid<W>(tokens, width, &grid, &block);
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, gather_bf16_kernel<W>, x, ld_x, row_of_slot, top_k, width, max_rows, out, ld_out),
+                "gather launch");
+}
+
+template <class W>
+int launch_combine(const uint16_t* rows, int64_t ld_rows, const int32_t* row_of_slot, const float* weights, int64_t tokens,
+                   int top_k, int width, int max_rows, uint16_t* y, int64_t ld_y, void* stream) {
+  dim3 grid, block;
+  row_grid<W>(tokens, width, &grid, &block);
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, combine_kernel<W>, rows, ld_rows, row_of_slot, weights, top_k, width, max_rows, y, ld_y),
+                "combine launch");
+}
+
+template <class W>
+int launch_combine_grad(const uint16_t* grad_y, int64_t ld_gy, const uint16_t* rows, int64_t ld_rows, const int32_t* row_of_slot,
+                        const float* weights, int64_t slots, int top_k, int width, int max_rows, uint16_t* grad_rows,
+                        int64_t ld_gr, float* grad_weights, void* stream) {
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((slots + kCta / 32 - 1) / (kCta / 32)), 1, 1), dim3(kCta, 1, 1),
+                                      0, static_cast<cudaStream_t>(stream), &attr);
+  return finish(cudaLaunchKernelEx(&cfg, combine_grad_kernel<W>, grad_y, ld_gy, rows, ld_rows, row_of_slot, weights, slots, top_k,
+                                   width, max_rows, grad_rows, ld_gr, grad_weights),
+                "combine backward launch");
 }
 
 }  // namespace
@@ -495,8 +539,14 @@ extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int t
   while (ctas < 8 && warps > 32 * ctas) ctas *= 2;
   warps = (warps + ctas - 1) / ctas;
   if (warps > 32) warps = 32;
+  p.sorters = warps;
   p.per_warp = static_cast<int>((p.n + static_cast<int64_t>(ctas) * warps * 32 - 1) / (static_cast<int64_t>(ctas) * warps * 32)) * 32;
   const size_t smem = static_cast<size_t>(warps + 3) * groups * sizeof(int);
+  // More warps where there are many groups or rows to walk at the end: 60 slots of 388 groups of 256 rows
+  // 22 us with the four that sort, 7 with 32.
+  const int64_t walk = align > 1 ? groups / 8 : 0;
+  const int64_t help = walk > max_rows / 512 ? walk : max_rows / 512;
+  const int all_warps = help <= warps ? warps : (help < 32 ? static_cast<int>(help) : 32);
   auto kernel = ctas > 1 ? dispatch_kernel<true> : dispatch_kernel<false>;
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -504,7 +554,7 @@ extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int t
     if (e != cudaSuccess) return set_cuda_error(e, "dispatch shared memory");
   }
   cudaLaunchAttribute attr[2];
-  cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, 1, 1), dim3(warps * 32, 1, 1), smem, static_cast<cudaStream_t>(stream), attr);
+  cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, 1, 1), dim3(all_warps * 32, 1, 1), smem, static_cast<cudaStream_t>(stream), attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(ctas);
   attr[1].val.clusterDim.y = 1;
@@ -521,14 +571,9 @@ extern "C" int smb_moe_gather_bf16_device(const uint16_t* x, int64_t ld_x, const
   if (ld_x < width || ld_out < width) return set_error(SMB_ERR_INVALID, "gather: pitch smaller than the row");
   if (!aligned_to(x, 2) || !aligned_to(out, 2)) return set_error(SMB_ERR_INVALID, "gather: rows are not 2-byte aligned");
   if (tokens == 0) return SMB_OK;
-  const bool al = aligned16(x, ld_x * 2) && aligned16(out, ld_out * 2);
-  dim3 grid, block;
-  row_grid(tokens, width, &grid, &block);
-  cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
-  return finish(cudaLaunchKernelEx(&cfg, al ? gather_bf16_kernel<true> : gather_bf16_kernel<false>, x, ld_x, row_of_slot, top_k,
-                                   width, static_cast<int>(max_rows), out, ld_out),
-                "gather launch");
+  auto take = [&](int n) { return rows_take(n, x, ld_x, width) && rows_take(n, out, ld_out, width); };
+  auto launch = take(16) ? launch_gather<uint4> : (take(4) ? launch_gather<uint32_t> : launch_gather<uint16_t>);
+  return launch(x, ld_x, row_of_slot, tokens, top_k, width, static_cast<int>(max_rows), out, ld_out, stream);
 }
 
 extern "C" int smb_moe_gather_i8_device(const uint16_t* x, int64_t ld_x, const int32_t* row_of_slot, int64_t tokens, int top_k,
@@ -546,7 +591,7 @@ extern "C" int smb_moe_gather_i8_device(const uint16_t* x, int64_t ld_x, const i
   const int64_t per_cta = warp ? kCta / 32 : 1;
   cudaLaunchAttribute attr;
   cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((tokens + per_cta - 1) / per_cta), 1, 1),
-                                      dim3(static_cast<unsigned>(warp ? kCta : qi8::row_threads(width, tokens)), 1, 1), 0,
+                                      dim3(static_cast<unsigned>(warp ? kCta : qi8::row_threads(width, tokens, al)), 1, 1), 0,
                                       static_cast<cudaStream_t>(stream), &attr);
   auto kernel = warp ? (al ? gather_i8_kernel<true, true> : gather_i8_kernel<true, false>)
                      : (al ? gather_i8_kernel<false, true> : gather_i8_kernel<false, false>);
@@ -564,14 +609,9 @@ extern "C" int smb_moe_combine_device(const uint16_t* rows, int64_t ld_rows, con
   if (!aligned_to(rows, 2) || !aligned_to(y, 2) || !aligned_to(weights, 4))
     return set_error(SMB_ERR_INVALID, "combine: rows must be 2-byte, weights 4-byte aligned");
   if (tokens == 0) return SMB_OK;
-  const bool al = aligned16(rows, ld_rows * 2) && aligned16(y, ld_y * 2);
-  dim3 grid, block;
-  row_grid(tokens, width, &grid, &block);
-  cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = pdl_config(grid, block, 0, static_cast<cudaStream_t>(stream), &attr);
-  return finish(cudaLaunchKernelEx(&cfg, al ? combine_kernel<true> : combine_kernel<false>, rows, ld_rows, row_of_slot, weights,
-                                   top_k, width, static_cast<int>(max_rows), y, ld_y),
-                "combine launch");
+  auto take = [&](int n) { return rows_take(n, rows, ld_rows, width) && rows_take(n, y, ld_y, width); };
+  auto launch = take(16) ? launch_combine<uint4> : (take(4) ? launch_combine<uint32_t> : launch_combine<uint16_t>);
+  return launch(rows, ld_rows, row_of_slot, weights, tokens, top_k, width, static_cast<int>(max_rows), y, ld_y, stream);
 }
 
 extern "C" int smb_moe_combine_backward_device(const uint16_t* grad_y, int64_t ld_grad_y, const uint16_t* rows,
@@ -589,15 +629,13 @@ extern "C" int smb_moe_combine_backward_device(const uint16_t* grad_y, int64_t l
       !aligned_to(grad_weights, 4))
     return set_error(SMB_ERR_INVALID, "combine backward: rows must be 2-byte, weights 4-byte aligned");
   if (tokens == 0) return SMB_OK;
-  const bool al = aligned16(grad_y, ld_grad_y * 2) && aligned16(grad_rows, ld_grad_rows * 2) &&
-                  (rows == nullptr || aligned16(rows, ld_rows * 2));
   const int64_t slots = tokens * top_k;
   if ((slots + kCta / 32 - 1) / (kCta / 32) > 0x7FFFFFFFLL) return set_error(SMB_ERR_UNSUPPORTED, "combine backward: too many slots");
-  cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((slots + kCta / 32 - 1) / (kCta / 32)), 1, 1), dim3(kCta, 1, 1),
-                                      0, static_cast<cudaStream_t>(stream), &attr);
-  return finish(cudaLaunchKernelEx(&cfg, al ? combine_grad_kernel<true> : combine_grad_kernel<false>, grad_y, ld_grad_y, rows,
-                                   ld_rows, row_of_slot, weights, slots, top_k, width, static_cast<int>(max_rows), grad_rows,
-                                   ld_grad_rows, grad_weights),
-                "combine backward launch");
+  auto take = [&](int n) {
+    return rows_take(n, grad_y, ld_grad_y, width) && rows_take(n, grad_rows, ld_grad_rows, width) &&
+           (grad_weights == nullptr || rows_take(n, rows, ld_rows, width));
+  };
+  auto launch = take(16) ? launch_combine_grad<uint4> : (take(4) ? launch_combine_grad<uint32_t> : launch_combine_grad<uint16_t>);
+  return launch(grad_y, ld_grad_y, rows, ld_rows, row_of_slot, weights, slots, top_k, width, static_cast<int>(max_rows),
+                grad_rows, ld_grad_rows, grad_weights, stream);
 }

@@ -26,7 +26,7 @@ quantize_i8_kernel(const void* src, int64_t ld_src, int8_t* codes, int64_t ld_by
   if (r >= rows) return;   // whole warps
   const void* row = static_cast<const char*>(src) + r * ld_src * (kBf16 ? 2 : 4);
   int8_t* out = codes + r * ld_bytes;
-  const float scale = qi8::quantize_row<kBf16, kWarp, kAligned>(
+  const float scale = qi8::quantize_row<kBf16, kWarp, kAligned, false>(
       row, K, tid, threads, red, [&](int k, uint2 c) { *reinterpret_cast<uint2*>(out + k) = c; },
       [&](int k, int8_t c) { out[k] = c; });
   if (tid == 0) scales[r] = scale;
@@ -42,7 +42,7 @@ cudaError_t launch_quantize(const cudaLaunchConfig_t& base, const void* src, int
     return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, true, kAligned>, src, ld_src, codes, ld_bytes, scales, rows, K);
   }
   cfg.gridDim = dim3(static_cast<unsigned>(rows), 1, 1);
-  cfg.blockDim = dim3(static_cast<unsigned>(qi8::row_threads(K, rows)), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(qi8::row_threads(K, rows, kAligned)), 1, 1);
   return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, false, kAligned>, src, ld_src, codes, ld_bytes, scales, rows, K);
 }
 

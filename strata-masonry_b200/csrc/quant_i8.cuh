@@ -102,40 +102,24 @@ __host__ __device__ inline RowScale row_scale(float amax, bool finite) {
 }
 
 constexpr int kHeldVecs = 4;      // vectors of a row that a thread keeps between the two passes
+constexpr int kHeldOnes = 16;     // the same where rows take no vectors, for a warp alone twice as many
 constexpr int kMaxRowWarps = 16;
 
 // Threads that share a row of K elements as a CTA of their own.  Many rows: as few as hold the row in registers,
 // since few threads with four vectors each keep more rows in flight than many with one (4095 x 4160 bf16 10.0
 // against 12.2 us).  Few rows: as many as there are vectors, for the shortest way through one row (rows
 // of 4096 for 16 tokens to 8 experts each, in the chain that sorts and sums them: 6.3 against 7.1 us).
-inline int row_threads(int64_t K, int64_t rows) {
-  const int vecs = rows <= 4 * 148 ? 1 : kHeldVecs;
+inline int row_threads(int64_t K, int64_t rows, bool aligned) {
+  const int vecs = rows <= 4 * 148 ? 1 : (aligned ? kHeldVecs : kHeldOnes / 8);
   int64_t t = (K / 8 + vecs - 1) / vecs;
   t = (t + 31) / 32 * 32;
   return static_cast<int>(t < 64 ? 64 : (t > kMaxRowWarps * 32 ? kMaxRowWarps * 32 : t));
 }
 
-// One row by `threads` threads: a warp (kWarp, no CTA barrier), or the whole CTA, `red` then holding a word
-// per warp.  `store8(k, codes)` and `store1(k, code)` receive the codes, after a barrier of the row's
-// threads; returns the row's scale.  Rows too long for the registers are read again (from L2).
-template <bool kBf16, bool kWarp, bool kAligned, class Store8, class Store1>
-__device__ __forceinline__ float quantize_row(const void* row, int K, int tid, int threads, uint32_t* red, Store8 store8,
-                                              Store1 store1) {
-  const int nvec = kAligned ? K / 8 : 0;
-  Vec<kBf16> held[kHeldVecs];
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < kHeldVecs; ++i) {
-    const int v = tid + i * threads;
-    if (v < nvec) held[i] = load_vec<kBf16>(row, static_cast<int64_t>(v) * 8);
-  }
-#pragma unroll
-  for (int i = 0; i < kHeldVecs; ++i)
-    if (tid + i * threads < nvec) m = abs_max_bits<kBf16>(held[i], m);
-  for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
-    m = abs_max_bits<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), m);
-  for (int k = nvec * 8 + tid; k < K; k += threads)
-    m = max(m, __float_as_uint(load_one<kBf16>(row, k)) & 0x7FFFFFFFu);
+// The largest magnitude over the threads of a row: a warp (kWarp, no CTA barrier), or the whole CTA, `red`
+// then holding a word per warp.
+template <bool kWarp>
+__device__ __forceinline__ RowScale join_max(uint32_t m, int tid, int threads, uint32_t* red) {
   m = __reduce_max_sync(0xffffffffu, m);
   __syncwarp();   // what the caller put into shared memory is there for store8 / store1
   if (!kWarp) {
@@ -144,17 +128,74 @@ __device__ __forceinline__ float quantize_row(const void* row, int K, int tid, i
     m = (tid & 31) < (threads >> 5) ? red[tid & 31] : 0u;
     m = __reduce_max_sync(0xffffffffu, m);
   }
-  const RowScale rs = row_scale(__uint_as_float(m), m < 0x7F800000u);
-  const float inv = rs.inv;
+  return row_scale(__uint_as_float(m), m < 0x7F800000u);
+}
+
+// One row by `threads` threads.  `store8(k, codes)` and `store1(k, code)` receive the codes, after a barrier
+// of the row's threads; returns the row's scale.  Rows too long for the registers are read again (from L2).
+// kAligned = false: rows on no 16-byte boundaries, an element a load and consecutive lanes on consecutive
+// elements, with as many loads in flight as the registers hold.  Bound by instructions: 4095 x 4161 bf16 23 us,
+// 4160 wide 9.9.
+// kMany: store1 is long, so what no thread needs of it is jumped over (a branch between short stores would
+// cost a third of the time).
+template <bool kBf16, bool kWarp, bool kAligned, bool kMany, class Store8, class Store1>
+__device__ __forceinline__ float quantize_row(const void* row, int K, int tid, int threads, uint32_t* red, Store8 store8,
+                                              Store1 store1) {
+  RowScale rs;
+  if constexpr (kAligned) {
+    const int nvec = K / 8;
+    Vec<kBf16> held[kHeldVecs];
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kHeldVecs; ++i) {
-    const int v = tid + i * threads;
-    if (v < nvec) store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(held[i], inv));
+    for (int i = 0; i < kHeldVecs; ++i) {
+      const int v = tid + i * threads;
+      if (v < nvec) held[i] = load_vec<kBf16>(row, static_cast<int64_t>(v) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeldVecs; ++i)
+      if (tid + i * threads < nvec) m = abs_max_bits<kBf16>(held[i], m);
+    for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
+      m = abs_max_bits<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), m);
+    for (int k = nvec * 8 + tid; k < K; k += threads)
+      m = max(m, __float_as_uint(load_one<kBf16>(row, k)) & 0x7FFFFFFFu);
+    rs = join_max<kWarp>(m, tid, threads, red);
+#pragma unroll
+    for (int i = 0; i < kHeldVecs; ++i) {
+      const int v = tid + i * threads;
+      if (v < nvec) store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(held[i], rs.inv));
+    }
+    for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
+      store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), rs.inv));
+    for (int k = nvec * 8 + tid; k < K; k += threads)
+      store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(load_one<kBf16>(row, k), rs.inv) & 0xFFu));
+  } else {
+    constexpr int kHeld = kWarp && !kMany ? 2 * kHeldOnes : kHeldOnes;
+    float held[kHeld];
+    auto load = [&](int k0) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) held[i] = k0 + i * threads < K ? load_one<kBf16>(row, k0 + i * threads) : 0.0f;
+    };
+    const int batch = kHeld * threads;
+    uint32_t m = 0;
+    for (int k0 = tid; k0 < K; k0 += batch) {
+      load(k0);
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) m = max(m, __float_as_uint(held[i]) & 0x7FFFFFFFu);
+    }
+    rs = join_max<kWarp>(m, tid, threads, red);
+    for (int k0 = tid; k0 < K; k0 += batch) {
+      if (K > batch) load(k0);
+#pragma unroll
+      for (int i0 = 0; i0 < kHeld; i0 += 4) {
+        if (kMany && k0 - tid + i0 * threads >= K) break;
+#pragma unroll
+        for (int i = i0; i < i0 + 4; ++i) {
+          const int k = k0 + i * threads;
+          if (k < K) store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(held[i], rs.inv) & 0xFFu));
+        }
+      }
+    }
   }
-  for (int v = tid + kHeldVecs * threads; v < nvec; v += threads)
-    store8(v * 8, rs.bad ? make_uint2(0, 0) : encode<kBf16>(load_vec<kBf16>(row, static_cast<int64_t>(v) * 8), inv));
-  for (int k = nvec * 8 + tid; k < K; k += threads)
-    store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(load_one<kBf16>(row, k), inv) & 0xFFu));
   return rs.bad ? __uint_as_float(0x7FC00000u) : rs.scale;
 }
 
