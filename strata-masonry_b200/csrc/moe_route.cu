@@ -41,8 +41,22 @@ struct RouteParams {
   float* weights;
   bool wide, bias_wide;   // rows of logits / the bias start on 16-byte boundaries
   int group_size;         // experts per group
-  int group_lanes;        // lanes per group where that is a power of two of whole lanes, else 0
+  int group_lanes;        // a power of two of lanes hold a group each; 0: lanes take no account of groups
 };
+
+// Lane sl of a token's segment holds the experts from lane_first on, at most V and up to lane_end; lower lanes
+// hold lower ones.  kSpread: groups are no whole numbers of full lanes, yet have lanes of their own.
+template <int V, bool kSpread>
+__device__ __forceinline__ int lane_first(const RouteParams& p, int sl) {
+  if (!kSpread) return sl * V;
+  const int shift = 31 - __clz(p.group_lanes);
+  return (sl >> shift) * p.group_size + (sl & (p.group_lanes - 1)) * V;
+}
+template <bool kSpread>
+__device__ __forceinline__ int lane_end(const RouteParams& p, int sl) {
+  if (!kSpread) return p.experts;
+  return min(p.experts, ((sl >> (31 - __clz(p.group_lanes))) + 1) * p.group_size);
+}
 
 // Bit patterns that order like the values.  Keys up to that of -inf stand for "closed".
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -123,10 +137,11 @@ __device__ __forceinline__ float load_logit(const void* row, int e) {
   return static_cast<const float*>(row)[e];
 }
 
-// V consecutive values from index e0 on, -inf beyond n.  `wide`: the row starts on a 16-byte boundary.
-template <int V, bool kBf16>
+// V consecutive values from index e0 on, -inf from n on.  `wide`: the row starts on a 16-byte boundary.
+template <int V, bool kBf16, bool kSpread = false>
 __device__ __forceinline__ void load_run(const void* row, int e0, int n, bool wide, float (&v)[V]) {
   constexpr int kPer = kBf16 ? 8 : 4;   // values in 16 bytes
+  if (kSpread) wide = wide && e0 % (V < kPer ? V : kPer) == 0;
   if (V % kPer == 0 && wide && e0 + V <= n) {
 #pragma unroll
     for (int i = 0; i < V / kPer; ++i) {
@@ -250,16 +265,16 @@ __device__ __noinline__ int choose_in_fp64(const RouteParams& p, const void* row
 // The open groups of the segments' tokens from fp64 scores.  The lane's V exponentials are independent of one
 // another, which is what keeps this short: a token in a thousand needs it, and the last of them sets the
 // kernel's end.
-template <int V, int L, bool kBf16>
+template <int V, int L, bool kBf16, bool kSpread>
 __device__ __noinline__ uint32_t groups_in_fp64(const RouteParams& p, const void* row, bool valid, double* buf, int lane) {
   const bool sigmoid = (p.flags & SMB_ROUTE_SIGMOID) != 0;
   const int sl = lane & (L - 1);
-  const int e0 = sl * V;
+  const int e0 = lane_first<V, kSpread>(p, sl), e_end = lane_end<kSpread>(p, sl);
   float l[V], b[V];
-  load_run<V, kBf16>(row, e0, valid ? p.experts : 0, p.wide, l);
+  load_run<V, kBf16, kSpread>(row, e0, valid ? e_end : 0, p.wide, l);
 #pragma unroll
   for (int i = 0; i < V; ++i) b[i] = 0.0f;
-  if (p.bias != nullptr) load_run<V, false>(p.bias, e0, p.experts, p.bias_wide, b);
+  if (p.bias != nullptr) load_run<V, false, kSpread>(p.bias, e0, e_end, p.bias_wide, b);
   float top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
@@ -386,7 +401,7 @@ __device__ __forceinline__ void sort_down(uint32_t (&k)[V]) {
 // the lane in the low bits of the key (two instructions per compare-exchange), and a choice is then one
 // maximum over the segment, one ballot and a shift of the winner's list.  The bits that the position covers
 // are made good like the rounding of exp: neighbours closer than their worth are settled in fp64.
-template <int V, int L, bool kBf16>
+template <int V, int L, bool kBf16, bool kSpread>
 __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(const RouteParams p) {
   constexpr int kTokens = 32 / L;   // per warp
   __shared__ double buf_all[kWarps][V * 32];
@@ -408,9 +423,9 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
   const bool by_score = p.bias != nullptr;
   const bool exact = kBf16 && !by_score;   // bf16 logits leave the low 16 bits of the key free
   constexpr uint32_t kPos = V <= 4 ? 3 : (V <= 8 ? 7 : 15);
-  const int e0 = sl * V;   // lanes hold runs of V experts, so lower lanes hold lower indices
+  const int e0 = lane_first<V, kSpread>(p, sl), e_end = lane_end<kSpread>(p, sl);
   float l[V];
-  load_run<V, kBf16>(row, e0, valid ? p.experts : 0, p.wide, l);
+  load_run<V, kBf16, kSpread>(row, e0, valid ? e_end : 0, p.wide, l);
   float top = 0.0f;
   if (sigmoid) {
 #pragma unroll
@@ -464,7 +479,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
     slack = 0x1p-23f * p_max * (sigmoid ? 6.0f + static_cast<float>(places) : 20.0f);
     if (by_score) {
       float b[V];
-      load_run<V, false>(p.bias, e0, p.experts, p.bias_wide, b);
+      load_run<V, false, kSpread>(p.bias, e0, e_end, p.bias_wide, b);
 #pragma unroll
       for (int i = 0; i < V; ++i) s[i] += b[i];
     }
@@ -480,7 +495,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
       float value = -INFINITY;   // lane g of the segment: value of group g
       const int lanes = p.group_lanes;
       if (lanes != 0) {
-        // A group is a run of 2^n whole lanes: join them by shuffles.  Keys of scores are sorted already.
+        // A group has 2^n lanes of its own: join them by shuffles.  Keys of scores are sorted already.
         if (by_score) {
           best.best = key_score(key[0] & ~kPos);
           best.second = key_score(key[1] & ~kPos);
@@ -521,7 +536,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
       const float v = key_value(last), w = key_value(first);
       // Sums of up to two scores, each with its rounding and hidden position bits.
       const bool tie = first > kClosedKey && v - w <= 2.0f * slack + 0x1p-23f * (kPos + 3) * (fabsf(v) + fabsf(w));
-      if (__any_sync(kFull, tie)) kept = groups_in_fp64<V, L, kBf16>(p, row, valid, buf_all[warp], lane);
+      if (__any_sync(kFull, tie)) kept = groups_in_fp64<V, L, kBf16, kSpread>(p, row, valid, buf_all[warp], lane);
       if (lanes != 0) {
         // A closed lane never wins, so its head alone keeps it out.
         if (!((kept >> ((sl >> (31 - __clz(lanes))) & 31)) & 1u)) key[0] = 0;
@@ -584,14 +599,14 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
       }
       __syncwarp();
       mine = sl < n ? won[sl].x : 0u;
-      id = mine != 0 ? static_cast<int>(won[sl].y * V + kPos - (mine & kPos)) : -1;
+      id = mine != 0 ? static_cast<int>(lane_first<V, kSpread>(p, won[sl].y) + kPos - (mine & kPos)) : -1;
       const int ordered = order_in_fp64<L, kBf16>(p, row, tie ? id : -1, tie ? n : 0, lane);
       if (tie) id = ordered;
       else if (sl >= p.top_k) id = -1;
       mine = 0;
     }
   }
-  if (mine != 0) id = static_cast<int>(won[sl].y * V + kPos - (mine & kPos));
+  if (mine != 0) id = static_cast<int>(lane_first<V, kSpread>(p, won[sl].y) + kPos - (mine & kPos));
   const unsigned again = __ballot_sync(kFull, close);
   if (again != 0) {
     __syncwarp();
@@ -786,24 +801,37 @@ int check_route(const void* logits, int dtype, int64_t ld, int tokens, int exper
   return SMB_OK;
 }
 
-// Lanes per token: as few as hold the experts, the choices (and two more that tie with the last) and the groups.  16384 tokens of 64 experts (bf16,
-// softmax, six choices), forward and backward: 16.6 us with a warp for every token, 9.5 with 8 lanes.  256
-// experts (sigmoid, bias, groups): 17.8 us with 32 lanes of 8, 20.0 with 16 lanes of 16.
+// Lanes of L with V experts each that a group gets if every group has a power of two of its own; 0: too few.
+int group_lanes(int V, int L, int experts, int n_groups) {
+  int lanes = 1;
+  while (lanes * V < experts / n_groups) lanes *= 2;
+  return lanes * n_groups <= L ? lanes : 0;
+}
+
+// Lanes per token: as few as hold the experts, the choices (and two more that tie with the last) and the
+// groups.  16384 tokens of 64 experts (bf16, softmax, six choices), forward and backward: 16.6 us with a warp
+// for every token, 9.5 with 8 lanes.  256 experts (sigmoid, bias, groups): 17.8 us with 32 lanes of 8, 20.0 with 16 lanes of 16.
 template <template <int, int, bool> class Launch, class P>
-int by_width(bool bf16, int experts, int lanes, const P& p, cudaStream_t st) {
-  if (experts > 256) return bf16 ? Launch<16, 32, true>::go(p, st) : Launch<16, 32, false>::go(p, st);
-  if (experts > 128 || lanes > 16) return bf16 ? Launch<8, 32, true>::go(p, st) : Launch<8, 32, false>::go(p, st);
-  if (experts > 64 || lanes > 8) return bf16 ? Launch<8, 16, true>::go(p, st) : Launch<8, 16, false>::go(p, st);
-  if (experts > 32) return bf16 ? Launch<8, 8, true>::go(p, st) : Launch<8, 8, false>::go(p, st);
-  return bf16 ? Launch<4, 8, true>::go(p, st) : Launch<4, 8, false>::go(p, st);
+int by_width(bool bf16, int experts, int lanes, int n_groups, const P& p, cudaStream_t st) {
+  // Every group on lanes of its own if that is possible at some width (17 groups of 30 it is not).
+  const bool whole = group_lanes(16, 32, experts, n_groups) != 0;
+  auto fits = [&](int v, int l) {
+    return experts <= v * l && lanes <= l && (n_groups == 1 || !whole || group_lanes(v, l, experts, n_groups) != 0);
+  };
+  if (fits(4, 8)) return bf16 ? Launch<4, 8, true>::go(p, st) : Launch<4, 8, false>::go(p, st);
+  if (fits(8, 8)) return bf16 ? Launch<8, 8, true>::go(p, st) : Launch<8, 8, false>::go(p, st);
+  if (fits(8, 16)) return bf16 ? Launch<8, 16, true>::go(p, st) : Launch<8, 16, false>::go(p, st);
+  if (fits(8, 32)) return bf16 ? Launch<8, 32, true>::go(p, st) : Launch<8, 32, false>::go(p, st);
+  return bf16 ? Launch<16, 32, true>::go(p, st) : Launch<16, 32, false>::go(p, st);
 }
 
 template <int V, int L, bool kBf16>
 struct LaunchRoute {
   static int go(RouteParams p, cudaStream_t st) {
-    const int lanes = p.group_size / V;
-    p.group_lanes = lanes * V == p.group_size && (lanes & (lanes - 1)) == 0 && lanes <= L ? lanes : 0;
-    return launch_tokens(route_kernel<V, L, kBf16>, p, 32 / L, st, "route launch");
+    p.group_lanes = p.top_groups < p.n_groups ? group_lanes(V, L, p.experts, p.n_groups) : 0;
+    auto kernel = p.group_lanes != 0 && p.group_lanes * V != p.group_size ? route_kernel<V, L, kBf16, true>
+                                                                          : route_kernel<V, L, kBf16, false>;
+    return launch_tokens(kernel, p, 32 / L, st, "route launch");
   }
 };
 template <int V, int L, bool kBf16>
@@ -841,7 +869,9 @@ extern "C" int smb_moe_route_device(const void* logits, int dtype, int64_t ld, c
   const RouteParams p = {logits, ld,    bias, tokens,  experts, top_k, n_groups, top_groups,
                          flags,  scale, ids,  weights, wide,    reinterpret_cast<uintptr_t>(bias) % 16 == 0,
                          experts / n_groups, 0};
-  return by_width<LaunchRoute>(dtype == SMB_DTYPE_BF16, experts, top_k + 2 > n_groups ? (top_k + 2 < 32 ? top_k + 2 : 32) : n_groups, p, static_cast<cudaStream_t>(stream));
+  const int lanes = top_k + 2 > n_groups ? (top_k + 2 < 32 ? top_k + 2 : 32) : n_groups;
+  return by_width<LaunchRoute>(dtype == SMB_DTYPE_BF16, experts, lanes, top_groups < n_groups ? n_groups : 1, p,
+                               static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int smb_moe_route_backward_device(const void* logits, int dtype, int64_t ld, const int32_t* ids,
@@ -863,5 +893,5 @@ extern "C" int smb_moe_route_backward_device(const void* logits, int dtype, int6
   auto rows_at = [](const void* q, int64_t bytes, int n) { return reinterpret_cast<uintptr_t>(q) % n == 0 && bytes % n == 0; };
   const RouteGradParams p = {logits, ld, ids, grad_weights, tokens, experts, top_k, flags, scale, grad_logits, ld_grad,
                              rows_at(logits, ld * size, 16), rows_at(grad_logits, ld_grad * size, 16)};
-  return by_width<LaunchRouteGrad>(dtype == SMB_DTYPE_BF16, experts, top_k, p, static_cast<cudaStream_t>(stream));
+  return by_width<LaunchRouteGrad>(dtype == SMB_DTYPE_BF16, experts, top_k, 1, p, static_cast<cudaStream_t>(stream));
 }
