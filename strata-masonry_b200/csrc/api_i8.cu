@@ -98,12 +98,13 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
   L.groups = g.groups;
   L.offsets = g.offsets;
   L.weights_static = (g.flags & SMB_FLAG_WEIGHTS_STATIC) != 0;
+  L.tma_store = g.ldd % 8 == 0 && reinterpret_cast<uintptr_t>(g.d) % 16 == 0 && !(g.flags & SMB_FLAG_FORCE_PLAIN_STORE);
   // Groups end inside a row tile: half a tile each on average.
-  i8_pick_tile(g.offsets != nullptr ? g.M + g.groups * 128 : g.M, g.N, g.K, device_cluster_slots(), &L.tile_n, &L.sub_blocks);
+  i8_pick_tile(g.offsets != nullptr ? g.M + g.groups * 128 : g.M, g.N, g.K, device_cluster_slots(), L.tma_store, &L.tile_n,
+               &L.sub_blocks);
   if (g.flags & SMB_FLAG_TILE_N_512) { L.tile_n = 256; L.sub_blocks = 2; }
   if (g.flags & SMB_FLAG_TILE_N_256) { L.tile_n = 256; L.sub_blocks = 1; }
   if (g.flags & SMB_FLAG_TILE_N_128) { L.tile_n = 128; L.sub_blocks = 1; }
-  L.tma_store = g.ldd % 8 == 0 && reinterpret_cast<uintptr_t>(g.d) % 16 == 0 && !(g.flags & SMB_FLAG_FORCE_PLAIN_STORE);
   int rc = SMB_OK;
   if (L.swiglu) {
     if (!L.tma_store)
@@ -112,7 +113,7 @@ int plan_create(smb_i8_plan** out, const I8Args& g, const void* act_src, int64_t
   }
   const bool tiled_only = (g.flags & (SMB_FLAG_NO_DECODE | SMB_FLAG_TILE_N_128 | SMB_FLAG_TILE_N_256 | SMB_FLAG_TILE_N_512)) != 0;
   L.decode = !tiled_only && i8_pick_decode(g.M, g.N, g.K, g.offsets != nullptr ? (g.groups < 2 ? 2 : g.groups) : 1,
-                                           (g.flags & SMB_FLAG_DECODE_SINGLE) != 0, &L.chunk, &L.box_rows);
+                                           L.tma_store, (g.flags & SMB_FLAG_DECODE_SINGLE) != 0, &L.chunk, &L.box_rows);
   if (act_src != nullptr && i8_decode_fuses(L, act_src, act_ld)) {
     L.x = static_cast<const uint16_t*>(act_src);
     L.ldx = act_ld;

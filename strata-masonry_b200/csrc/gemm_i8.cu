@@ -433,19 +433,29 @@ int launch_i8_store(const I8Launch& L, cudaStream_t stream) {
 
 }  // namespace
 
-// Estimated cycles of the three tiles, waves x K blocks x cycles per K block.  A stage of 24, 32 or 48 KB takes
-// 400, 540 or 1084 cycles (the first two are the 64 bytes per cycle that an SM takes in through TMA); the
-// 512-wide tile adds 2500 cycles of accumulator drain and runs at a higher clock for its smaller traffic.
+// Estimated cycles of the three tiles.  A K block (24, 32 or 48 KB) takes 630, 756 or 1432 cycles in a chain of
+// launches (from the 64 bytes per cycle that an SM takes in through TMA, at the clock that their power leaves);
+// draining and storing a tile takes 14 cycles a column, 29 without TMA stores, half hidden (three quarters
+// with TMA) behind the next tile's K loop.  The 512-wide tile has no second accumulator: only loads hide its
+// drain, from the second wave on.
 // Measured, us, 128 / 256 / 512 wide: 256 x 4096 x 4096 11.2 / 14.9 / 25.5, 256 x 28672 x 8192 70 / 58 / 59,
-// 4095 x 12289 x 4160 - / 146 / 151.
-void i8_pick_tile(int M, int N, int K, int clusters, int* tile_n, int* sub_blocks) {
+// 1151 x 4040 x 90 6.6 / 7.9 / 8.8, 1000 deep 12.6 / 11.9 / 13.5; without TMA stores 4095 x 12289 x 4160 198 / 146 /
+// 180, 1151 x 4039 x 90 9.4 / 11.7 / 13.7.
+void i8_pick_tile(int M, int N, int K, int clusters, bool tma_store, int* tile_n, int* sub_blocks) {
   if (clusters < 1) clusters = 74;
   const long long tiles_m = (M + 255) / 256;
   const long long kb = (K + 127) / 128;
+  const double column = tma_store ? 14.0 : 29.0;
   auto waves = [&](int width) { return static_cast<double>((tiles_m * ((N + width - 1) / width) + clusters - 1) / clusters); };
-  const double cost128 = waves(128) * kb * 400.0;
-  const double cost256 = waves(256) * kb * 540.0;
-  const double cost512 = waves(512) * (kb * 1084.0 + 2500.0) / 1.06;
+  auto cost = [&](int width, double block) {
+    const double loop = kb * block, drain = width * column;
+    const double more = loop < drain ? loop : drain, open = tma_store ? 0.25 : 0.5;
+    return waves(width) * (loop + drain - more + open * more) + (1.0 - open) * more;
+  };
+  const double cost128 = cost(128, 630.0), cost256 = cost(256, 756.0);
+  const double loop512 = kb * 1432.0, drain512 = 512 * column;
+  const double shown = (drain512 > loop512 ? drain512 - loop512 : 0.0) + (tma_store ? 2500.0 : 8000.0);
+  const double cost512 = waves(512) * (loop512 + shown) - shown + 0.85 * drain512;
   *tile_n = cost128 <= cost256 && cost128 <= cost512 ? 128 : 256;
   *sub_blocks = *tile_n == 256 && cost512 < cost256 ? 2 : 1;
 }

@@ -546,14 +546,50 @@ int launch_i8_decode(const I8Launch& L, const i8d::Params& p, int ctas, int spli
   return SMB_OK;
 }
 
+int usable_sms() {
+  const int slots = device_cluster_slots();
+  return slots > 0 ? 2 * slots : 148;
+}
+
+// CTAs that share the K loop of a tile: with SMs to spare, the number of the lowest estimate in cycles, the K
+// blocks at the 48 bytes per cycle that reach a CTA from HBM and the exchange of the sums, which is short
+// where they are pushed.  us with 1 / 2 / 4 CTAs: 48 x 1024 x 512 3.9 / 6.1 / -, 64 x 1024 x 1024 - / 7.5 / 6.1.
+// (As many as fill both places of every SM: 1 x 4096 x 4096 from bf16 7.3 instead of 6.6 us, 128 x 4096 x 4096
+// 12.7 instead of 11.3.)
+int k_split(long long tiles, int K, int chunk, int sms, int* kb_per) {
+  const int num_kb = (K + i8d::kBlockK - 1) / i8d::kBlockK;
+  const bool push = chunk <= i8d::kPushTokens;
+  const int block = (i8d::kWBytes + chunk * i8d::kBlockK) / 48;
+  int best = 1, best_cost = num_kb * block;
+  for (int split = 2; split <= i8d::kMaxSplit && tiles * split <= sms && num_kb >= 2 * split; split *= 2) {
+    const int cost = (num_kb + split - 1) / split * block + (push ? 800 + chunk / split * 60 : 1500 + chunk / split * 130);
+    if (cost < best_cost) {
+      best = split;
+      best_cost = cost;
+    }
+  }
+  *kb_per = (num_kb + best - 1) / best;
+  return (num_kb + *kb_per - 1) / *kb_per;
+}
+
 }  // namespace
 
-bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows) {
+bool i8_pick_decode(int M, int N, int K, int groups, bool tma_store, bool force, int* chunk, int* box_rows) {
   if (groups == 1) {
     // us here / best tiled kernel: 128 x 28672 x 8192 43 / 56, 128 x 4096 x 4096 11.3 / 14.1, 128 x 1024 x 8192
     // 9.6 / 16.5, but 64 x 8192 x 2048 9.3 / 8.2: a short K loop over enough 128-wide tiles for most clusters
     // leaves little to gain over 64 rows.
-    if (M > 128 && !force) return false;
+    if (M > 128 && !force) {
+      // A few tiles with a long K, which only this kernel cuts: cycles of 256 x 128 tiles on as many clusters
+      // against a share of the K loop and the exchange of 128 x 128 sums.  us tiled / here: 209 x 43 x 5141
+      // 12.6 / 7.8, 1024 x 256 x 8192 16.1 / 11.3, 256 x 1024 x 4096 9.9 / 10.1, 2048 x 512 x 8192 17 / 24.
+      const long long tiles = static_cast<long long>((M + 127) / 128) * ((N + 127) / 128);
+      int kb_per = 0;
+      const int split = k_split(tiles, K, 128, usable_sms(), &kb_per);
+      if (split == 1) return false;
+      const int num_kb = (K + i8d::kBlockK - 1) / i8d::kBlockK;
+      if (num_kb * 400 + (tma_store ? 1800 : 3700) <= kb_per * 680 + 7500 + 128 / split * 130) return false;
+    }
     if (M >= 64 && N >= 8192 && K <= 2048 && !force) return false;
     *chunk = M >= 128 ? 128 : (M + 15) / 16 * 16;
     *box_rows = *chunk;
@@ -571,16 +607,6 @@ bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int
 }
 
 namespace {
-
-// K split: as many CTAs per tile as SMs are free, at least two K blocks each.  (As many as fill both places of
-// every SM: 1 x 4096 x 4096 from bf16 7.3 instead of 6.6 us, 128 x 4096 x 4096 12.7 instead of 11.3.)
-int k_split(long long tiles, int K, int sms, int* kb_per) {
-  const int num_kb = (K + i8d::kBlockK - 1) / i8d::kBlockK;
-  int split = 1;
-  while (split < i8d::kMaxSplit && tiles * split * 2 <= sms && num_kb >= split * 4) split *= 2;
-  *kb_per = (num_kb + split - 1) / split;
-  return (num_kb + *kb_per - 1) / *kb_per;
-}
 
 template <int kSplit, bool kFused>
 int launch_store(const I8Launch& L, const i8d::Params& p, int ctas, int split, cudaStream_t stream) {
@@ -623,7 +649,7 @@ int i8_decode_launch(const I8Launch& L, cudaStream_t stream) {
   if (L.offsets != nullptr) chunks = L.M / L.chunk + (L.groups < L.M ? L.groups : L.M);
   const long long tiles = chunks * p.tiles_n;
   if (tiles > 0x7FFFFFFFLL) return set_error(SMB_ERR_UNSUPPORTED, "i8 decode: too many tiles");
-  const int split = k_split(tiles, L.K, L.x != nullptr ? all_sms : sms, &p.kb_per);   // as the plan decided
+  const int split = k_split(tiles, L.K, L.x != nullptr ? i8d::kFusedRows : L.chunk, L.x != nullptr ? all_sms : sms, &p.kb_per);   // as the plan decided
   long long ctas;
   if (split > 1) {
     ctas = tiles * split;
@@ -662,8 +688,7 @@ bool i8_decode_fuses(const I8Launch& L, const void* x, long long ldx) {
       reinterpret_cast<uintptr_t>(x) % 16 != 0)
     return false;
   int kb_per = 0;
-  const int slots = device_cluster_slots();
-  k_split((L.N + i8d::kTileRows - 1) / i8d::kTileRows, L.K, slots > 0 ? 2 * slots : 148, &kb_per);
+  k_split((L.N + i8d::kTileRows - 1) / i8d::kTileRows, L.K, i8d::kFusedRows, usable_sms(), &kb_per);
   return kb_per <= i8d::kFusedMaxBlocks;
 }
 

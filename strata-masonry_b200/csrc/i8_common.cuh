@@ -36,10 +36,10 @@ struct I8Launch {
   int* status;
 };
 
-void i8_pick_tile(int M, int N, int K, int clusters, int* tile_n, int* sub_blocks);
+void i8_pick_tile(int M, int N, int K, int clusters, bool tma_store, int* tile_n, int* sub_blocks);
 int i8_launch(const I8Launch& L, cudaStream_t stream);
 // Whether the decode kernel is taken for M rows in `groups` groups, with its chunk and box heights.
-bool i8_pick_decode(int M, int N, int K, int groups, bool force, int* chunk, int* box_rows);
+bool i8_pick_decode(int M, int N, int K, int groups, bool tma_store, bool force, int* chunk, int* box_rows);
 int i8_decode_launch(const I8Launch& L, cudaStream_t stream);
 bool i8_decode_fuses(const I8Launch& L, const void* x, long long ldx);   // for plain plans fed with bf16 rows
 
