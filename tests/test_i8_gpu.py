@@ -110,6 +110,42 @@ def test_i8_extreme_codes_do_not_wrap(smb, cuda_device):
     _check(torch, d, _sums(torch, a, b, k), sa, sb)
 
 
+@pytest.mark.parametrize("shape", [(209, 43, 5141), (1024, 256, 8192), (296, 189, 3759), (48, 1024, 512), (64, 1024, 1024),
+                                   (100, 512, 1024), (33, 2048, 2048), (1, 1024, 512), (16, 1024, 640), (555, 7452, 190),
+                                   (1151, 4039, 90), (150, 2694, 1972)])
+def test_i8_choice_of_kernel_and_split(smb, cuda_device, shape):
+    """On either side of the rules that cut the K loop or pick a tile width; forced the other way, the bits agree."""
+    torch = _torch()
+    m, n, k = shape
+    a, sa, b, sb, d = _run(smb, torch, m, n, k)
+    _check(torch, d, _sums(torch, a, b, k), sa, sb)
+    for flag in (smb.capi.FLAG_NO_DECODE, smb.capi.FLAG_DECODE_SINGLE):
+        assert torch.equal(_run(smb, torch, m, n, k, flags=flag)[4].view(torch.int16), d.view(torch.int16))
+
+
+@pytest.mark.parametrize("n", [64, 130, 191, 256, 321])
+@pytest.mark.parametrize("pad", [0, 1, 2, 3])
+@pytest.mark.parametrize("tile", ["FLAG_TILE_N_128", "FLAG_TILE_N_256", "FLAG_TILE_N_512"])
+def test_i8_plain_store_alignments(smb, cuda_device, n, pad, tile):
+    """Whole boxes by pairs and by elements, boxes that end inside M or N, from a base of odd elements too."""
+    torch = _torch()
+    m, k = 301, 160
+    a, b = _codes(torch, m, k, 7), _codes(torch, n, k, 8)
+    sa, sb = _scales(torch, m, 9), _scales(torch, n, 10)
+    want = _expect_bits(torch, _sums(torch, a, b, k), sa, sb)
+    ldd = n + pad
+    for shift in (0, 1, 2):
+        buf = torch.full((shift + m * ldd + 8,), 9.0, device="cuda", dtype=torch.bfloat16)
+        d = buf[shift:shift + m * ldd].view(m, ldd)
+        flags = getattr(smb.capi, tile) | smb.capi.FLAG_FORCE_PLAIN_STORE
+        plan = smb.gemm.I8Plan(a, sa, b, sb, d, m, n, k, lda=a.shape[1], ldb=b.shape[1], ldd=ldd, flags=flags)
+        plan.run()
+        plan.check()
+        plan.close()
+        assert torch.equal(d[:, :n].view(torch.int16), want.view(torch.int16))
+        assert bool((d[:, n:] == 9).all()) and bool((buf[:shift] == 9).all()) and bool((buf[shift + m * ldd:] == 9).all())
+
+
 @pytest.mark.parametrize("m", [5, 300])
 @pytest.mark.parametrize("ldd", [104, 101])
 def test_i8_pitched_output_keeps_its_padding(smb, cuda_device, m, ldd):
@@ -399,3 +435,24 @@ def test_i8_random_shapes_all_schedules_agree(smb, cuda_device, seed):
         _check(torch, outs[0], _sums(torch, a, b, k), sa, sb)
         for d in outs[1:]:
             assert torch.equal(d.view(torch.int16), outs[0].view(torch.int16)), (m, n, k)
+
+
+@pytest.mark.parametrize("case", [(5, 33), (7, 511), (3, 1023), (700, 1025), (2, 8190), (900, 2046), (9, 16500), (601, 8195)])
+@pytest.mark.parametrize("bf16", [True, False])
+def test_i8_quantizer_rows_without_vectors(smb, cuda_device, case, bf16):
+    torch = _torch()
+    rows, k = case
+    g = torch.Generator(device="cuda")
+    g.manual_seed(k)
+    x = torch.randn(rows, k, generator=g, device="cuda") * torch.exp(torch.randn(rows, 1, generator=g, device="cuda"))
+    x = x.bfloat16() if bf16 else x
+    x[1, k - 1] = float("inf")
+    codes = torch.full((rows, k + 3), 55, device="cuda", dtype=torch.int8)
+    scales = torch.empty(rows, device="cuda")
+    call = smb.gemm.quantize_i8_bf16_device if bf16 else smb.gemm.quantize_i8_device
+    call(x, codes, scales, rows, k, ld_bytes=k + 3)
+    torch.cuda.synchronize()
+    want_c, want_s = smb.gemm.quantize_i8_host(x.float().cpu().numpy())
+    np.testing.assert_array_equal(codes[:, :k].cpu().numpy(), want_c)
+    np.testing.assert_array_equal(scales.cpu().numpy(), want_s)
+    assert bool((codes[:, k:] == 55).all())

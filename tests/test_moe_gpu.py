@@ -169,6 +169,35 @@ def test_route_extreme_logits(smb, cuda_device):
     np.testing.assert_allclose(w.cpu().numpy(), [[1, np.exp(-50)]], rtol=2 ** -17)
 
 
+# Groups that are no whole number of a lane's experts, and one whose lanes do not suffice for lanes of their own.
+GROUP_CASES = [(70, 36, 8, 2, 1), (300, 160, 6, 8, 3), (65, 144, 6, 8, 3), (40, 48, 6, 8, 1), (33, 16, 2, 8, 3), (20, 304, 4, 8, 2),
+               (31, 240, 7, 12, 5), (29, 510, 8, 17, 6), (50, 21, 3, 7, 3), (17, 62, 9, 31, 8), (12, 12, 6, 4, 2)]
+
+
+@pytest.mark.parametrize("case", GROUP_CASES, ids=str)
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("pad", [0, 3, 8])
+def test_route_groups_of_any_size(smb, cuda_device, case, bf16, pad):
+    torch = _torch()
+    tokens, experts, top_k, n_groups, top_groups = case
+    rng = np.random.default_rng(experts + pad)
+    l = _logits(rng, tokens, experts)
+    l[1] = -np.inf
+    l[2, :experts // 2] = np.nan
+    l[3:8] = np.round(l[3:8])                    # ties inside and between groups
+    c = smb.capi
+    for bias in (None, (0.1 * rng.standard_normal(experts)).astype(np.float32)):
+        for sigmoid in (False, True):
+            for top2 in (False, True):
+                flags = ((c.ROUTE_SIGMOID if sigmoid else 0) | c.ROUTE_RENORM | (c.ROUTE_GROUP_TOP2 if top2 else 0))
+                buf, ids, weights = _route(smb, torch, l, c.DTYPE_BF16 if bf16 else c.DTYPE_F32, top_k, bias, n_groups,
+                                           top_groups, flags, 2.5, pad=pad)
+                want_ids, want = _route_plain(buf[:, :experts].float().cpu().numpy().astype(np.float64), bias, top_k, n_groups,
+                                              top_groups, sigmoid, True, top2, 2.5)
+                np.testing.assert_array_equal(ids.cpu().numpy(), want_ids)
+                assert np.all(np.abs(weights.cpu().numpy() - want) <= np.abs(want) * 2.0 ** -17)
+
+
 @pytest.mark.parametrize("sigmoid", [False, True])
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("experts", [16, 64, 256, 512])
@@ -330,6 +359,26 @@ def test_dispatch_against_plain(smb, cuda_device, case, skew):
         assert (got[len(w_tiles):cap // 256] == groups - 1).all()
 
 
+@pytest.mark.parametrize("case", [(10, 6, 388, 256), (3, 2, 1024, 512), (700, 4, 1024, 128), (1, 1, 1, 65536), (60, 1, 33, 4096)],
+                         ids=str)
+def test_dispatch_with_more_rows_than_slots(smb, cuda_device, case):
+    """Few slots, many padded rows and groups: warps without slots help to walk them."""
+    torch = _torch()
+    tokens, top_k, groups, align = case
+    rng = np.random.default_rng(groups)
+    ids = rng.integers(-1, groups, size=(tokens, top_k)).astype(np.int32)
+    tile_map = align % 256 == 0
+    cap, offsets, row_of_slot, slot_of_row, tiles = _dispatch(smb, torch, ids, groups, align, 7000, tile_map)
+    w_off, w_row, w_slot, w_tiles = _dispatch_plain(ids, groups, align, cap)
+    np.testing.assert_array_equal(offsets.cpu().numpy(), w_off)
+    np.testing.assert_array_equal(row_of_slot.cpu().numpy(), w_row)
+    np.testing.assert_array_equal(slot_of_row.cpu().numpy(), w_slot)
+    if tile_map:
+        got = tiles.cpu().numpy()
+        np.testing.assert_array_equal(got[:len(w_tiles)], w_tiles)
+        assert (got[len(w_tiles):cap // 256] == groups - 1).all()
+
+
 def _bf16(torch, *shape, seed):
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
@@ -409,6 +458,48 @@ def test_combine_and_its_gradients(smb, cuda_device, case, weighted):
     got = g_rows[:cap][live[:cap]][:, :width].double()
     assert bool(((got - ref_r).abs() <= (2.0 ** -8 + 2 * U) * ref_r.abs()).all())
     assert bool((g_rows[~live[:cap]] == 9).all()) and bool((g_rows[:, width:] == 9).all())
+
+
+@pytest.mark.parametrize("width,shift,pad", [(2048, 0, 0), (2048, 1, 0), (2048, 0, 2), (2046, 0, 0), (2046, 2, 0), (2047, 0, 0),
+                                             (2047, 0, 1), (700, 4, 4), (33, 3, 0), (5000, 1, 1)])
+def test_rows_of_any_alignment(smb, cuda_device, width, shift, pad):
+    """Rows in words of 16, 4 and 2 bytes: bases shifted by elements, odd pitches and widths."""
+    torch = _torch()
+    tokens, top_k, groups = 19, 9, 7
+    cap, _, row_of_slot, slot_of_row = _map(smb, torch, tokens, top_k, groups, width + shift)
+    ld = width + pad
+
+    def rows(n, fill=None, seed=0):
+        buf = torch.full((n * ld + shift,), 9.0, device="cuda", dtype=torch.bfloat16) if fill else _bf16(torch, n * ld + shift, seed=seed)
+        return buf[shift:].view(n, ld)
+
+    x, out, e, y, g = rows(tokens, seed=1), rows(cap, fill=True), rows(cap, seed=2), rows(tokens, fill=True), rows(cap, fill=True)
+    weights, gw = torch.rand(tokens, top_k, device="cuda"), torch.full((tokens, top_k), 9.0, device="cuda")
+    codes = torch.full((cap, ld), 55, device="cuda", dtype=torch.int8)
+    scales = torch.full((cap,), 55.0, device="cuda")
+    args = (tokens, top_k, width, cap)
+    smb.moe.gather_bf16_device(x, row_of_slot, out, *args, ld_x=ld, ld_out=ld)
+    smb.moe.gather_i8_device(x, row_of_slot, codes, scales, *args, ld_x=ld, ld_bytes=ld)
+    smb.moe.combine_device(e, row_of_slot, weights, y, *args, ld_rows=ld, ld_y=ld)
+    smb.moe.combine_backward_device(x, e, row_of_slot, weights, g, gw, *args, ld_grad_y=ld, ld_rows=ld, ld_grad_rows=ld)
+    torch.cuda.synchronize()
+    live = slot_of_row >= 0
+    slot = slot_of_row[live].long()
+    token = slot // top_k
+    assert torch.equal(out[live[:cap]][:, :width], x[token][:, :width])
+    assert bool((out[~live[:cap]] == 9).all()) and bool((out[:, width:] == 9).all())
+    want_c, want_s = smb.gemm.quantize_i8_host(x[:, :width].float().cpu().numpy())
+    np.testing.assert_array_equal(codes[live[:cap]].cpu().numpy()[:, :width], want_c[token.cpu().numpy()])
+    np.testing.assert_array_equal(scales[live[:cap]].cpu().numpy(), want_s[token.cpu().numpy()])
+    have = row_of_slot >= 0
+    picked = torch.where(have[:, :, None], e[row_of_slot.long().clamp_min(0)][:, :, :width].double(), 0.0)
+    terms = picked * weights.double()[:, :, None]
+    assert bool(((y[:, :width].double() - terms.sum(1)).abs() <= 2.0 ** -8 * terms.sum(1).abs() + (top_k + 1) * U * terms.abs().sum(1)).all())
+    prod = picked * x[:, None, :width].double()
+    assert bool(((gw.double() - prod.sum(2)).abs() <= (width / 32 + 16) * U * prod.abs().sum(2)).all())
+    ref = x[token][:, :width].double() * weights.reshape(-1)[slot].double()[:, None]
+    assert bool(((g[live[:cap]][:, :width].double() - ref).abs() <= (2.0 ** -8 + 2 * U) * ref.abs()).all())
+    assert bool((g[~live[:cap]] == 9).all()) and bool((y[:, width:] == 9).all())
 
 
 def test_rows_outside_the_buffer_are_skipped(smb, cuda_device):
