@@ -28,6 +28,8 @@ struct StoreTarget {
   float alpha;                 // factor on every accumulator (kScaled instantiations only)
   int row_end;                 // rows >= row_end are not written (a tile's share of a ragged group;
                                // M where tiles own whole boxes)
+  bool keep_padding = false;   // TMA path: D is left alone between N and the next 16-byte boundary of a row,
+                               // up to which a TMA store writes
 };
 
 // One warp drains kCols fp32 columns of its 32 TMEM lanes starting at `taddr`, then writes them
@@ -168,7 +170,20 @@ __device__ __forceinline__ void store_columns(const uint32_t (&packed)[kOutCols 
                    packed[c * 32 + 4 * j + 2], packed[c * 32 + 4 * j + 3]);
     }
     const int gcol0 = col0 + c * kStoreCols;
-    if (kTmaStore) {
+    if (kTmaStore && out.keep_padding && out.N % 8 != 0 && gcol0 + kStoreCols > out.N) {
+      // The last box of a row: element by element, in as few registers as that takes.
+      __syncwarp();
+      const int rows = min(32, min(out.M, out.row_end) - row0);
+      uint16_t* dst = out.d_ptr + static_cast<size_t>(row0) * out.ldd + gcol0;
+#pragma unroll 1
+      for (int i = lane; i < rows * kStoreCols; i += 32) {
+        const int r = i / kStoreCols, cc = i % kStoreCols;
+        uint16_t v;
+        asm volatile("ld.shared.u16 %0, [%1];"
+                     : "=h"(v) : "r"(sbuf + r * 128 + ((((cc >> 3) ^ (r & 7)) << 4) | ((cc & 7) << 1))) : "memory");
+        if (gcol0 + cc < out.N) dst[static_cast<size_t>(r) * out.ldd + cc] = v;
+      }
+    } else if (kTmaStore) {
       fence_proxy_async_smem();
       __syncwarp();
       const int n_peers = out.peers->count;

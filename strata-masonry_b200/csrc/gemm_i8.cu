@@ -303,6 +303,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant
     out.N = kSwiglu ? p.N / 2 : p.N;
     out.peers = &p.peers;
     out.alpha = 1.0f;
+    out.keep_padding = true;
     int local = 0;
     for (int t = cluster; t < num_tiles; t += n_clusters, ++local) {
       int tm, tn;

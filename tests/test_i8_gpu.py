@@ -146,6 +146,37 @@ def test_i8_plain_store_alignments(smb, cuda_device, n, pad, tile):
         assert bool((d[:, n:] == 9).all()) and bool((buf[:shift] == 9).all()) and bool((buf[shift + m * ldd:] == 9).all())
 
 
+@pytest.mark.parametrize("n", [1, 7, 30, 66, 130, 381, 514])
+@pytest.mark.parametrize("tile", ["FLAG_NONE", "FLAG_TILE_N_128", "FLAG_TILE_N_256", "FLAG_TILE_N_512", "FLAG_DECODE_SINGLE"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_i8_columns_of_a_wider_matrix(smb, cuda_device, n, tile, gated):
+    """D is the left part of a matrix whose other columns belong to someone else: a row that ends inside 16
+    bytes ends there, in tiles and in ragged groups."""
+    torch = _torch()
+    n += n % 2 if gated else 0
+    wide, k, groups = n // 2 if gated else n, 96, 3
+    ldd = (wide + 7) // 8 * 8 + 8
+    flags = getattr(smb.capi, tile) | (smb.capi.FLAG_EPILOGUE_SWIGLU if gated else 0)
+    for m, cuts in ((40, None), (300, None), (333, [0, 70, 71, 330])):
+        a, b = _codes(torch, m, k, 11), _codes(torch, groups * n, k, 12)
+        sa, sb = _scales(torch, m, 13), _scales(torch, groups * n, 14)
+        d = torch.full((m, ldd), 7.0, device="cuda", dtype=torch.bfloat16)
+        args = dict(lda=a.shape[1], ldb=b.shape[1], ldd=ldd, flags=flags)
+        if cuts is None:
+            plan = smb.gemm.I8Plan(a, sa, b, sb, d, m, n, k, **args)
+        else:
+            offsets = torch.tensor(cuts, device="cuda", dtype=torch.int32)
+            plan = smb.gemm.I8Plan.grouped(a, sa, b, sb, d, m, n, k, groups, offsets, **args)
+        plan.run()
+        plan.check()
+        plan.close()
+        for g, (lo, hi) in enumerate(zip(*((cuts[:-1], cuts[1:]) if cuts else ([0], [m])))):
+            acc = _sums(torch, a[lo:hi], b[g * n:(g + 1) * n], k)
+            check = _check_gated if gated else _check
+            check(torch, d[lo:hi, :wide], acc, sa[lo:hi], sb[g * n:(g + 1) * n])
+        assert bool((d[:, wide:] == 7).all()) and (cuts is None or bool((d[cuts[-1]:] == 7).all()))
+
+
 @pytest.mark.parametrize("m", [5, 300])
 @pytest.mark.parametrize("ldd", [104, 101])
 def test_i8_pitched_output_keeps_its_padding(smb, cuda_device, m, ldd):
