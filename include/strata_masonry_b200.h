@@ -433,8 +433,8 @@ int smb_fp4_host_ctx_create_sharded(smb_fp4_host_ctx** ctx, int M, int n_local, 
  *   D[m,n] = bf16_rne( (float(sum_k A[m,k] B[n,k]) * sa[m]) * sb[n] ),  the sum exact in int32.
  * A [M,K] and B [N,K] are int8, row-major, row pitches multiples of 16 bytes, base pointers 16-byte
  * aligned; sa [M] and sb [N] are fp32; D is bf16 row-major, of any 2-byte alignment and
- * pitch (rows on 16-byte boundaries are stored faster); what lies behind the N columns of a row is left
- * alone.
+ * pitch (rows on 16-byte boundaries are stored faster, and the gated epilogue needs them); what lies behind
+ * the columns of a row is left alone.
  * Any M, N from 1 to 2^30 and 1 <= K <= 131071 (the int32 sum of 131072 products could wrap).  No reference
  * counterpart: its int8 path is not part of the dense GEMM tree.
  * ---------------------------------------------------------------------------------- */

@@ -11,7 +11,8 @@
 // Bound by the tensor cores, from a second of load on by the 1 kW power cap: 8192^3 in 311 us (3.53 PFLOP/s, the
 // tensor pipe busy 91 % of the cycles) in bursts and 366 us (3.0 PFLOP/s) sustained, 2.1 times the bf16
 // rate either way; DRAM reads 340 MB of 134 MB of operands.  A grouped launch of 64 experts x 32768 rows (gated,
-// 4096 x 2048 each) takes 239 us / 279 us sustained: 161 row tiles where 128 full ones would do.
+// 4096 x 2048 each) takes 230 to 240 us / 287 us sustained: 161 row tiles where 128 full ones would do.  With a
+// K below about 768 the epilogue bounds it, 5.6K cycles for a 256 x 256 tile.
 //
 // Rounding: the int32 sum becomes fp32 (half a step, 2^-24 relative), two fp32 products follow
 // (2^-24 each), one rounding to bf16 (2^-8) ends it.
@@ -440,8 +441,8 @@ int launch_i8_store(const I8Launch& L, cudaStream_t stream) {
 // with TMA) behind the next tile's K loop.  The 512-wide tile has no second accumulator: only loads hide its
 // drain, from the second wave on.
 // Measured, us, 128 / 256 / 512 wide: 256 x 4096 x 4096 11.2 / 14.9 / 25.5, 256 x 28672 x 8192 70 / 58 / 59,
-// 1151 x 4040 x 90 6.6 / 7.9 / 8.8, 1000 deep 12.6 / 11.9 / 13.5; without TMA stores 4095 x 12289 x 4160 198 / 146 /
-// 180, 1151 x 4039 x 90 9.4 / 11.7 / 13.7.
+// 1151 x 4040 x 90 6.9 / 8.1 / 9.0, 1000 deep 12.6 / 12.0 / 13.5; without TMA stores 4095 x 12289 x 4160 200 / 146 /
+// 173, 1151 x 4039 x 90 8.6 / 10.5 / 10.6.
 void i8_pick_tile(int M, int N, int K, int clusters, bool tma_store, int* tile_n, int* sub_blocks) {
   if (clusters < 1) clusters = 74;
   const long long tiles_m = (M + 255) / 256;
