@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kCta) gather_bf16_kernel(const uint16_t* x, in
   }
 }
 
-template <bool kWarp, bool kAligned>
+template <bool kWarp, int kPer>
 __global__ void __launch_bounds__(kWarp ? kCta : 32 * qi8::kMaxRowWarps)
 gather_i8_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int64_t tokens, int top_k, int width, int max_rows,
                  int8_t* codes, int64_t ld_bytes, float* scales) {
@@ -276,12 +276,18 @@ gather_i8_kernel(const uint16_t* x, int64_t ld_x, const int* row_of_slot, int64_
   // its stores.
   int* rows = rows_all[kWarp ? threadIdx.x >> 5 : 0];
   if (tid < top_k) rows[tid] = row_of_slot[t * top_k + tid];
-  const float scale = qi8::quantize_row<true, kWarp, kAligned, true>(
+  const float scale = qi8::quantize_row<true, kWarp, kPer, true>(
       x + t * ld_x, width, tid, threads, red,
       [&](int k, uint2 c) {
         for (int j = 0; j < top_k; ++j) {
           const int r = rows[j];
           if (r >= 0 && r < max_rows) *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(r) * ld_bytes + k) = c;
+        }
+      },
+      [&](int k, uint16_t c) {
+        for (int j = 0; j < top_k; ++j) {
+          const int r = rows[j];
+          if (r >= 0 && r < max_rows) *reinterpret_cast<uint16_t*>(codes + static_cast<int64_t>(r) * ld_bytes + k) = c;
         }
       },
       [&](int k, int8_t c) {
@@ -418,7 +424,6 @@ __global__ void __launch_bounds__(kCta) combine_grad_kernel(const uint16_t* grad
   }
 }
 
-bool aligned16(const void* p, int64_t ld_bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld_bytes % 16 == 0; }
 // Whether rows of 2-byte elements consist of words of n bytes.
 bool rows_take(int n, const void* p, int64_t ld, int width) {
   return reinterpret_cast<uintptr_t>(p) % n == 0 && ld * 2 % n == 0 && static_cast<int64_t>(width) * 2 % n == 0;
@@ -586,15 +591,15 @@ extern "C" int smb_moe_gather_i8_device(const uint16_t* x, int64_t ld_x, const i
   if (!aligned_to(x, 2) || !aligned_to(scales, 4))
     return set_error(SMB_ERR_INVALID, "i8 gather: rows must be 2-byte, scales 4-byte aligned");
   if (tokens == 0) return SMB_OK;
-  const bool al = aligned16(x, ld_x * 2) && aligned_to(codes, 8) && ld_bytes % 8 == 0;
+  const int per = qi8::row_per(x, ld_x, codes, ld_bytes, width, true);
   const bool warp = width <= 1024;   // a warp holds such a row in registers
   const int64_t per_cta = warp ? kCta / 32 : 1;
   cudaLaunchAttribute attr;
   cudaLaunchConfig_t cfg = pdl_config(dim3(static_cast<unsigned>((tokens + per_cta - 1) / per_cta), 1, 1),
-                                      dim3(static_cast<unsigned>(warp ? kCta : qi8::row_threads(width, tokens, al)), 1, 1), 0,
+                                      dim3(static_cast<unsigned>(warp ? kCta : qi8::row_threads(width, tokens, per)), 1, 1), 0,
                                       static_cast<cudaStream_t>(stream), &attr);
-  auto kernel = warp ? (al ? gather_i8_kernel<true, true> : gather_i8_kernel<true, false>)
-                     : (al ? gather_i8_kernel<false, true> : gather_i8_kernel<false, false>);
+  auto kernel = warp ? (per == 8 ? gather_i8_kernel<true, 8> : (per == 2 ? gather_i8_kernel<true, 2> : gather_i8_kernel<true, 1>))
+                     : (per == 8 ? gather_i8_kernel<false, 8> : (per == 2 ? gather_i8_kernel<false, 2> : gather_i8_kernel<false, 1>));
   return finish(cudaLaunchKernelEx(&cfg, kernel, x, ld_x, row_of_slot, tokens, top_k, width, static_cast<int>(max_rows), codes,
                                    ld_bytes, scales),
                 "i8 gather launch");

@@ -14,7 +14,7 @@ namespace {
 constexpr int kWarpRows = 8;        // rows of a CTA where a warp takes a row
 constexpr int kWarpMaxK = 1024;     // ... which it holds in registers
 
-template <bool kBf16, bool kWarp, bool kAligned>
+template <bool kBf16, bool kWarp, int kPer>
 __global__ void __launch_bounds__(kWarp ? 32 * kWarpRows : 32 * qi8::kMaxRowWarps)
 quantize_i8_kernel(const void* src, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales, int64_t rows, int K) {
   __shared__ uint32_t red[qi8::kMaxRowWarps];
@@ -26,24 +26,25 @@ quantize_i8_kernel(const void* src, int64_t ld_src, int8_t* codes, int64_t ld_by
   if (r >= rows) return;   // whole warps
   const void* row = static_cast<const char*>(src) + r * ld_src * (kBf16 ? 2 : 4);
   int8_t* out = codes + r * ld_bytes;
-  const float scale = qi8::quantize_row<kBf16, kWarp, kAligned, false>(
+  const float scale = qi8::quantize_row<kBf16, kWarp, kPer, false>(
       row, K, tid, threads, red, [&](int k, uint2 c) { *reinterpret_cast<uint2*>(out + k) = c; },
+      [&](int k, uint16_t c) { *reinterpret_cast<uint16_t*>(out + k) = c; },
       [&](int k, int8_t c) { out[k] = c; });
   if (tid == 0) scales[r] = scale;
 }
 
-template <bool kBf16, bool kAligned>
+template <bool kBf16, int kPer>
 cudaError_t launch_quantize(const cudaLaunchConfig_t& base, const void* src, int64_t ld_src, int8_t* codes,
                             int64_t ld_bytes, float* scales, int64_t rows, int K) {
   cudaLaunchConfig_t cfg = base;
   if (K <= kWarpMaxK) {
     cfg.gridDim = dim3(static_cast<unsigned>((rows + kWarpRows - 1) / kWarpRows), 1, 1);
     cfg.blockDim = dim3(32 * kWarpRows, 1, 1);
-    return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, true, kAligned>, src, ld_src, codes, ld_bytes, scales, rows, K);
+    return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, true, kPer>, src, ld_src, codes, ld_bytes, scales, rows, K);
   }
   cfg.gridDim = dim3(static_cast<unsigned>(rows), 1, 1);
-  cfg.blockDim = dim3(static_cast<unsigned>(qi8::row_threads(K, rows, kAligned)), 1, 1);
-  return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, false, kAligned>, src, ld_src, codes, ld_bytes, scales, rows, K);
+  cfg.blockDim = dim3(static_cast<unsigned>(qi8::row_threads(K, rows, kPer)), 1, 1);
+  return cudaLaunchKernelEx(&cfg, quantize_i8_kernel<kBf16, false, kPer>, src, ld_src, codes, ld_bytes, scales, rows, K);
 }
 
 int check_quantize(const void* src, int64_t ld_src, const void* codes, int64_t ld_bytes, const void* scales, int64_t rows,
@@ -62,9 +63,10 @@ int check_quantize(const void* src, int64_t ld_src, const void* codes, int64_t l
 int quantize_i8_launch(const void* src, bool bf16, int64_t ld_src, int8_t* codes, int64_t ld_bytes, float* scales,
                        int64_t rows, int64_t K, cudaStream_t st) {
   if (rows == 0) return SMB_OK;
-  const int size = bf16 ? 2 : 4;
-  const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0 && (ld_src * size) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(codes) % 8 == 0 && ld_bytes % 8 == 0;
+  int per = qi8::row_per(src, ld_src, codes, ld_bytes, K, bf16);
+  // A warp a row: pairs win by throughput alone.  us by elements / by pairs: 1026 x 162 2.1 / 2.9, 1026 x 1002 2.7 /
+  // 3.6, 4000 x 602 3.9 / 3.9, 16000 x 162 10.5 / 7.8, 16000 x 1002 28 / 11.4.
+  if (per == 2 && K <= kWarpMaxK && rows <= 4000) per = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
   cudaLaunchAttribute pdl;
@@ -75,11 +77,12 @@ int quantize_i8_launch(const void* src, bool bf16, int64_t ld_src, int8_t* codes
   const int k = static_cast<int>(K);
   cudaError_t e;
   if (bf16)
-    e = aligned ? launch_quantize<true, true>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
-                : launch_quantize<true, false>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
+    e = per == 8 ? launch_quantize<true, 8>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
+        : per == 2 ? launch_quantize<true, 2>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
+                   : launch_quantize<true, 1>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
   else
-    e = aligned ? launch_quantize<false, true>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
-                : launch_quantize<false, false>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
+    e = per == 8 ? launch_quantize<false, 8>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k)
+                 : launch_quantize<false, 1>(cfg, src, ld_src, codes, ld_bytes, scales, rows, k);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "i8 quantize launch");
   return SMB_OK;

@@ -102,18 +102,26 @@ __host__ __device__ inline RowScale row_scale(float amax, bool finite) {
 }
 
 constexpr int kHeldVecs = 4;      // vectors of a row that a thread keeps between the two passes
-constexpr int kHeldOnes = 16;     // the same where rows take no vectors, for a warp alone twice as many
+constexpr int kHeldWords = 16;    // the same where rows take no vectors, for a warp with single elements twice as many
 constexpr int kMaxRowWarps = 16;
 
 // Threads that share a row of K elements as a CTA of their own.  Many rows: as few as hold the row in registers,
 // since few threads with four vectors each keep more rows in flight than many with one (4095 x 4160 bf16 10.0
 // against 12.2 us).  Few rows: as many as there are vectors, for the shortest way through one row (rows
 // of 4096 for 16 tokens to 8 experts each, in the chain that sorts and sums them: 6.3 against 7.1 us).
-inline int row_threads(int64_t K, int64_t rows, bool aligned) {
-  const int vecs = rows <= 4 * 148 ? 1 : (aligned ? kHeldVecs : kHeldOnes / 8);
-  int64_t t = (K / 8 + vecs - 1) / vecs;
+// Elements a load: 8 (rows on 16-byte boundaries), 2 (bf16 on 4-byte ones, an even number of them) or 1.
+inline int row_threads(int64_t K, int64_t rows, int per) {
+  const int elems = rows <= 4 * 148 ? 8 : (per == 8 ? 8 * kHeldVecs : (per == 2 ? 32 : 16));
+  int64_t t = (K + elems - 1) / elems;
   t = (t + 31) / 32 * 32;
   return static_cast<int>(t < 64 ? 64 : (t > kMaxRowWarps * 32 ? kMaxRowWarps * 32 : t));
+}
+
+inline int row_per(const void* src, int64_t ld_src, const void* codes, int64_t ld_bytes, int64_t K, bool bf16) {
+  const uintptr_t s = reinterpret_cast<uintptr_t>(src), c = reinterpret_cast<uintptr_t>(codes);
+  const int64_t pitch = ld_src * (bf16 ? 2 : 4);
+  if (s % 16 == 0 && pitch % 16 == 0 && c % 8 == 0 && ld_bytes % 8 == 0) return 8;
+  return bf16 && s % 4 == 0 && pitch % 4 == 0 && c % 2 == 0 && ld_bytes % 2 == 0 && K % 2 == 0 ? 2 : 1;
 }
 
 // The largest magnitude over the threads of a row: a warp (kWarp, no CTA barrier), or the whole CTA, `red`
@@ -131,18 +139,18 @@ __device__ __forceinline__ RowScale join_max(uint32_t m, int tid, int threads, u
   return row_scale(__uint_as_float(m), m < 0x7F800000u);
 }
 
-// One row by `threads` threads.  `store8(k, codes)` and `store1(k, code)` receive the codes, after a barrier
-// of the row's threads; returns the row's scale.  Rows too long for the registers are read again (from L2).
-// kAligned = false: rows on no 16-byte boundaries, an element a load and consecutive lanes on consecutive
-// elements, with as many loads in flight as the registers hold.  Bound by instructions: 4095 x 4161 bf16 23 us,
-// 4160 wide 9.9.
-// kMany: store1 is long, so what no thread needs of it is jumped over (a branch between short stores would
-// cost a third of the time).
-template <bool kBf16, bool kWarp, bool kAligned, bool kMany, class Store8, class Store1>
+// One row by `threads` threads.  `store8(k, codes)`, `store2(k, codes)` and `store1(k, code)` receive the codes,
+// after a barrier of the row's threads; returns the row's scale.  Rows too long for the registers are read
+// again (from L2).  kPer = 2 and 1: rows on no 16-byte boundaries, a pair or an element a load and consecutive
+// lanes on consecutive ones, with as many loads in flight as the registers hold.  Bound by instructions: 4095
+// rows of 4161 bf16 23 us, of 4162 15.6, of 4160 9.9.
+// kMany: the stores are long, so what no thread needs of them is jumped over (a branch between short stores
+// would cost a third of the time).
+template <bool kBf16, bool kWarp, int kPer, bool kMany, class Store8, class Store2, class Store1>
 __device__ __forceinline__ float quantize_row(const void* row, int K, int tid, int threads, uint32_t* red, Store8 store8,
-                                              Store1 store1) {
+                                              Store2 store2, Store1 store1) {
   RowScale rs;
-  if constexpr (kAligned) {
+  if constexpr (kPer == 8) {
     const int nvec = K / 8;
     Vec<kBf16> held[kHeldVecs];
     uint32_t m = 0;
@@ -169,29 +177,44 @@ __device__ __forceinline__ float quantize_row(const void* row, int K, int tid, i
     for (int k = nvec * 8 + tid; k < K; k += threads)
       store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(load_one<kBf16>(row, k), rs.inv) & 0xFFu));
   } else {
-    constexpr int kHeld = kWarp && !kMany ? 2 * kHeldOnes : kHeldOnes;
-    float held[kHeld];
-    auto load = [&](int k0) {
+    static_assert(kPer == 1 || kBf16, "pairs of bf16");
+    constexpr int kHeld = kWarp && !kMany && kPer == 1 ? 2 * kHeldWords : kHeldWords;
+    const int words = K / kPer;
+    uint32_t held[kHeld];   // a pair, or the bits of a float
+    auto load = [&](int w0) {
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) held[i] = k0 + i * threads < K ? load_one<kBf16>(row, k0 + i * threads) : 0.0f;
+      for (int i = 0; i < kHeld; ++i) {
+        const int w = w0 + i * threads;
+        if (kPer == 2) held[i] = w < words ? static_cast<const uint32_t*>(row)[w] : 0u;
+        else held[i] = w < words ? __float_as_uint(load_one<kBf16>(row, w)) : 0u;
+      }
     };
     const int batch = kHeld * threads;
     uint32_t m = 0;
-    for (int k0 = tid; k0 < K; k0 += batch) {
-      load(k0);
+    for (int w0 = tid; w0 < words; w0 += batch) {
+      load(w0);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) m = max(m, __float_as_uint(held[i]) & 0x7FFFFFFFu);
+      for (int i = 0; i < kHeld; ++i)
+        m = kPer == 2 ? __vmaxu2(m, held[i] & 0x7FFF7FFFu) : max(m, held[i] & 0x7FFFFFFFu);
     }
+    if (kPer == 2) m = max(m << 16, m & 0xFFFF0000u);
     rs = join_max<kWarp>(m, tid, threads, red);
-    for (int k0 = tid; k0 < K; k0 += batch) {
-      if (K > batch) load(k0);
+    for (int w0 = tid; w0 < words; w0 += batch) {
+      if (words > batch) load(w0);
 #pragma unroll
       for (int i0 = 0; i0 < kHeld; i0 += 4) {
-        if (kMany && k0 - tid + i0 * threads >= K) break;
+        if (kMany && w0 - tid + i0 * threads >= words) break;
 #pragma unroll
         for (int i = i0; i < i0 + 4; ++i) {
-          const int k = k0 + i * threads;
-          if (k < K) store1(k, rs.bad ? 0 : static_cast<int8_t>(code_bits(held[i], rs.inv) & 0xFFu));
+          const int w = w0 + i * threads;
+          if (w >= words) continue;
+          if (kPer == 2) {
+            const uint32_t lo = code_bits(__uint_as_float(held[i] << 16), rs.inv) & 0xFFu;
+            const uint32_t hi = code_bits(__uint_as_float(held[i] & 0xFFFF0000u), rs.inv) & 0xFFu;
+            store2(2 * w, rs.bad ? uint16_t(0) : static_cast<uint16_t>(lo | hi << 8));
+          } else {
+            store1(w, rs.bad ? 0 : static_cast<int8_t>(code_bits(__uint_as_float(held[i]), rs.inv) & 0xFFu));
+          }
         }
       }
     }

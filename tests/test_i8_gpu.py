@@ -468,7 +468,7 @@ def test_i8_random_shapes_all_schedules_agree(smb, cuda_device, seed):
             assert torch.equal(d.view(torch.int16), outs[0].view(torch.int16)), (m, n, k)
 
 
-@pytest.mark.parametrize("case", [(5, 33), (7, 511), (3, 1023), (700, 1025), (2, 8190), (900, 2046), (9, 16500), (601, 8195)])
+@pytest.mark.parametrize("case", [(5, 33), (7, 511), (3, 1023), (700, 1025), (2, 8190), (900, 2046), (9, 16500), (601, 8195), (4100, 66), (5000, 1022)])
 @pytest.mark.parametrize("bf16", [True, False])
 def test_i8_quantizer_rows_without_vectors(smb, cuda_device, case, bf16):
     torch = _torch()
