@@ -109,7 +109,6 @@ constexpr int kMaxRowWarps = 16;
 // since few threads with four vectors each keep more rows in flight than many with one (4095 x 4160 bf16 10.0
 // against 12.2 us).  Few rows: as many as there are vectors, for the shortest way through one row (rows
 // of 4096 for 16 tokens to 8 experts each, in the chain that sorts and sums them: 6.3 against 7.1 us).
-// Elements a load: 8 (rows on 16-byte boundaries), 2 (bf16 on 4-byte ones, an even number of them) or 1.
 inline int row_threads(int64_t K, int64_t rows, int per) {
   const int elems = rows <= 4 * 148 ? 8 : (per == 8 ? 8 * kHeldVecs : (per == 2 ? 32 : 16));
   int64_t t = (K + elems - 1) / elems;
@@ -117,6 +116,7 @@ inline int row_threads(int64_t K, int64_t rows, int per) {
   return static_cast<int>(t < 64 ? 64 : (t > kMaxRowWarps * 32 ? kMaxRowWarps * 32 : t));
 }
 
+// Elements a load: 8 (rows on 16-byte boundaries), 2 (bf16 on 4-byte ones, an even number of them) or 1.
 inline int row_per(const void* src, int64_t ld_src, const void* codes, int64_t ld_bytes, int64_t K, bool bf16) {
   const uintptr_t s = reinterpret_cast<uintptr_t>(src), c = reinterpret_cast<uintptr_t>(codes);
   const int64_t pitch = ld_src * (bf16 ? 2 : 4);
