@@ -71,6 +71,7 @@ struct Cfg {
   static constexpr int kColsPerWarp = TN / kGroupsPerSlot;
   static constexpr int kSlotReaders = 2 * 4 * kGroupsPerSlot;    // arrivals per drained slot
   static_assert(kTotal <= (kResident == 2 ? 115712 : 232448), "shared memory budget");
+  static_assert(kTotal >= kHolderShared, "least of a holder of tensor memory");
   static_assert(kStages >= 2 && kStages <= 16, "ring depth");
 };
 
@@ -135,7 +136,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
 
   // Programmatic dependent launch: the next kernel on the stream may begin its prologue while
   // this grid is still running (it waits, below, before it loads or stores anything).
-  griddep_launch_dependents();
+  if (fills_sm(C::kTotal)) griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full_bar(s), 1);    // the leader's arrive.expect_tx covers both CTAs' bytes
@@ -160,6 +161,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmap_a,
   }
   tc_fence_before_sync();
   __syncthreads();
+  if (!fills_sm(C::kTotal)) griddep_launch_dependents();   // not before this CTA holds its tensor memory
   cluster_sync_all();
   tc_fence_after_sync();
   uint32_t tmem_base;

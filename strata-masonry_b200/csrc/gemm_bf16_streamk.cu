@@ -45,6 +45,7 @@ constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kStoreBytes = kEpiWarps * kStoreBufBytes;
 constexpr int kTotal = 1024 + kRingBytes + kStoreBytes + 1024;
 static_assert(kTotal <= 232448, "shared memory budget");
+static_assert(fills_sm(kTotal), "the next kernel starts before the allocation");
 
 struct Params {
   int M, N, K;

@@ -32,6 +32,17 @@ int comm_device(const smb_comm* comm);
 // long it waited.  Stream-ordered.  selftest.cu.
 int wait_probe_launch(int* status, long long budget_cycles, long long* waited_cycles, cudaStream_t stream);
 
+// --------------------------------------------------------------------------- tensor memory
+// Every kernel takes its tensor memory without a limit on the wait, and lets the next kernel on the stream start
+// while it runs.  That one may take tensor memory on the same SM and keep it until its own wait for this
+// kernel ends, so an allocation that comes after the start of the next kernel could wait for good.  Two
+// rules exclude it: a kernel that leaves room for another holder on its SM starts the next one only when it has
+// allocated; one that fills its SM may do so at once, which is up to 0.3 us sooner (2048^3 bf16, launched one by one:
+// 15.9 against 16.2 us).
+constexpr int kSmShared = 228 * 1024;        // shared memory of an SM; 1 KB of it is set aside for each CTA
+constexpr int kHolderShared = 96 * 1024;     // no kernel that holds tensor memory takes less
+constexpr bool fills_sm(int shared) { return shared + kHolderShared + 2 * 1024 > kSmShared; }
+
 // --------------------------------------------------------------------------- raster
 // Map a flat tile index onto (tile_m, tile_n).  Tiles are walked in groups of `group_m`
 // tile rows; inside a group the M index runs fastest.  With ~74 clusters working on

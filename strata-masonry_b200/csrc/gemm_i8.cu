@@ -50,6 +50,7 @@ struct Cfg {
   static constexpr int kColsPerWarp = TN / kGroupsPerSlot;
   static constexpr int kSlotReaders = 2 * 4 * kGroupsPerSlot;      // arrivals per drained slot
   static_assert(kTotal <= 232448, "shared memory budget");
+  static_assert(fills_sm(kTotal), "the next kernel starts before the allocation");
 };
 
 struct Params {

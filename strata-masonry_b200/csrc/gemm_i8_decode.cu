@@ -47,6 +47,7 @@ constexpr int kTableBytes = (kI8MaxGroups + 8) * 4;
 // CTA that holds some may be waiting for the very kernel that asks for more.  (Of the other kernels that
 // allocate it, the narrow BF16 and FP4 tiles take half an SM of both; the rest leave no room beside them.)
 constexpr int kTotal = 111 * 1024;
+static_assert(kTotal >= kHolderShared, "least of a holder of tensor memory");
 constexpr int kRingBudget = kTotal - 1024 - kBarBytes - kTableBytes;
 
 struct Params {

@@ -86,6 +86,7 @@ struct Cfg {
   static_assert(kColsPerWarp % kStoreCols == 0, "epilogue split");
   static_assert(kAccCols + kStages * kSlotCols <= kTmemCols, "tensor memory budget");
   static_assert(kTotal <= (R == 2 ? 115712 : 232448), "shared memory budget");
+  static_assert(kTotal >= kHolderShared, "least of a holder of tensor memory");
   static_assert(kStages >= 2, "ring depth");
 };
 
@@ -189,7 +190,7 @@ gemm_nvfp4_kernel(const __grid_constant__ CUtensorMap tmap_a,
 
   // Programmatic dependent launch: the next kernel on the stream may begin its prologue while
   // this grid is still running (it waits, below, before it loads or stores anything).
-  griddep_launch_dependents();
+  if (fills_sm(C::kTotal)) griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -219,6 +220,7 @@ gemm_nvfp4_kernel(const __grid_constant__ CUtensorMap tmap_a,
   }
   tc_fence_before_sync();
   __syncthreads();
+  if (!fills_sm(C::kTotal)) griddep_launch_dependents();   // not before this CTA holds its tensor memory
   cluster_sync_all();
   tc_fence_after_sync();
   uint32_t tmem_base;

@@ -57,6 +57,7 @@ constexpr int kSlotCols = kCells * 4 + kBands * kCells * 4;
 static_assert(kStageBytes % 1024 == 0 && kOffRing % 1024 == 0, "ring stages must stay 1024-byte aligned");
 static_assert(kAccCols + kStages * kSlotCols <= 512, "tensor memory budget");
 static_assert(kTotal <= 232448, "shared memory budget");
+static_assert(fills_sm(kTotal), "the next kernel starts before the allocation");
 
 struct Params {
   int M, N, K;

@@ -45,10 +45,11 @@ constexpr int kWBytes = 128 * kBlockKBytes;   // 16 KiB weight box
 constexpr int kSfBytes = 1024;        // one 128-row band x 8 scales (two 512-byte cells)
 constexpr int kSlotCols = 16;         // SFW cells (8 columns) + SFX cells (8 columns) per stage
 constexpr int kMaxStages = 16;
-// These kernels take all 512 columns of tensor memory after they have let the next kernel start.  More than
-// half of an SM's shared memory, however few stages are asked for, keeps that kernel's tensor memory (which it
-// may hold while it waits for this one) off their SMs.
+// At least this much shared memory, however few stages are asked for: more than half of what an SM has, so that
+// two CTAs of a launch never share one.  Each takes all 512 columns of tensor memory, so the second would only
+// start once the first is through, and where the grid quantises the activations as a whole the first waits for it.
 constexpr int kMinSmem = 118 * 1024;
+static_assert(kMinSmem >= kHolderShared, "least of a holder of tensor memory");
 constexpr int kDefaultStages = 6;
 constexpr int kDualFromPad = 16;      // padded activation rows from which two tiles share one activation box
 constexpr int kWholeTileStages = 8;
@@ -125,9 +126,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& tmap_w, const CUt
   const uint32_t sfw_off = kWBytes + static_cast<uint32_t>(p.m_pad) * kBlockKBytes;
   const uint32_t sfx_off = sfw_off + kSfBytes;
 
-  // Let the next launch on the stream start its prologue and its (read-only) operand loads
-  // while this grid is still running; it waits before it touches D or the scratch.
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -154,6 +152,10 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& tmap_w, const CUt
   }
   tc_fence_before_sync();
   __syncthreads();
+  // Let the next launch on the stream start its prologue and its (read-only) operand loads
+  // while this grid is still running; it waits before it touches D or the scratch.  Not before this CTA
+  // holds its tensor memory: the next kernel may take its own on this SM and keep it while it waits.
+  griddep_launch_dependents();
   tc_fence_after_sync();
   uint32_t tmem_base;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
@@ -728,7 +730,6 @@ __device__ __forceinline__ void decode_dual_body(const CUtensorMap& tmap_w, cons
   const int epi_groups = p.m_pad >= 32 ? 2 : 1;
   const int cols_group0 = ((p.m_pad / 16 + 1) / 2) * 16;
 
-  griddep_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), kFused ? 2 : 1);      // TMA producer (+ the quantising warp of the stage)
@@ -756,6 +757,7 @@ __device__ __forceinline__ void decode_dual_body(const CUtensorMap& tmap_w, cons
   }
   tc_fence_before_sync();
   __syncthreads();
+  griddep_launch_dependents();   // not before this CTA holds its tensor memory
   tc_fence_after_sync();
   uint32_t tmem_base;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot) : "memory");
