@@ -54,7 +54,8 @@ struct DispatchParams {
 // One cluster sorts everything: warp w of the cluster owns the slots [w * per_warp, + per_warp), so
 // "earlier slots" means earlier lanes, earlier chunks, earlier warps, earlier CTAs, and the counts of the
 // CTAs meet through distributed shared memory instead of a second launch.
-//   shared: hist[sorters][groups] | total[groups] | start[groups] | count[groups]
+//   shared: hist[sorters][groups] | total[groups] | start[groups] | count[groups] | warp_sums[32], all of it asked
+//   for by the launch, since what a kernel declares itself counts towards the 48 KB that need no asking too
 // Bound by latency: the ids of a warp are fetched together (8 x 32 at a time) and stay in registers
 // between the count and the placement where they fit.  128 slots of 256 groups 2.3 us, 4096 of 64 4.3 us; 65536
 // slots 9.8 us on the eight SMs of a cluster, where the copies that follow take 190.
@@ -77,7 +78,6 @@ __device__ __forceinline__ unsigned same_id(int e, int bits) {
 template <bool kCluster>
 __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) {
   extern __shared__ int sm[];
-  __shared__ int warp_sums[32];
   griddep_launch_dependents();
   const int all_warps = blockDim.x >> 5, warps = p.sorters;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(1024) dispatch_kernel(const DispatchParams p) 
   int* total = hist + warps * G;
   int* start = total + G;
   int* count = start + G;
+  int* warp_sums = count + G;
 
   const long long first = warp < warps ? static_cast<long long>(rank * warps + warp) * p.per_warp : p.n;
   const int lo = static_cast<int>(first < p.n ? first : p.n);
@@ -546,7 +547,8 @@ extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int t
   if (warps > 32) warps = 32;
   p.sorters = warps;
   p.per_warp = static_cast<int>((p.n + static_cast<int64_t>(ctas) * warps * 32 - 1) / (static_cast<int64_t>(ctas) * warps * 32)) * 32;
-  const size_t smem = static_cast<size_t>(warps + 3) * groups * sizeof(int);
+  auto shared = [](int sorters, int groups) { return (static_cast<size_t>(sorters + 3) * groups + 32) * sizeof(int); };
+  const size_t smem = shared(warps, groups);
   // More warps where there are many groups or rows to walk at the end: 60 slots of 388 groups of 256 rows
   // 22 us with the four that sort, 7 with 32.
   const int64_t walk = align > 1 ? groups / 8 : 0;
@@ -555,7 +557,7 @@ extern "C" int smb_moe_dispatch_device(const int32_t* ids, int64_t tokens, int t
   auto kernel = ctas > 1 ? dispatch_kernel<true> : dispatch_kernel<false>;
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         35 * kMaxDispatchGroups * static_cast<int>(sizeof(int)));
+                                         static_cast<int>(shared(32, kMaxDispatchGroups)));
     if (e != cudaSuccess) return set_cuda_error(e, "dispatch shared memory");
   }
   cudaLaunchAttribute attr[2];

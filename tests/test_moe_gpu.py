@@ -6,8 +6,12 @@ the divisions and the scale a handful: below 128 u = 2^-17 relative.  Gradients 
 so 2^-16 of the sum of the terms' magnitudes, plus 2^-8 relative where they are stored in bf16.
 Weighted sums: top_k fused multiply-adds (u each of the running magnitude) and one rounding to bf16.
 """
+from pathlib import Path
+
 import numpy as np
 import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
 
 pytestmark = pytest.mark.gpu
 
@@ -700,3 +704,27 @@ def test_rows_on_another_stream(smb, cuda_device):
     stream.synchronize()
     # Weights add up to one, every copy is the token itself.
     assert bool(((y.double() - x.double()).abs() <= 2.0 ** -8 * x.double().abs() + 64 * U * x.double().abs()).all())
+
+
+def test_dispatch_histograms_just_below_the_default_shared_memory(tmp_path):
+    """Histograms of 47.9 to 48 KB, in a process whose first calls they are: nothing has raised the kernel's limit
+    before.  The last case sorts on a cluster."""
+    import subprocess
+    import sys
+    script = tmp_path / "first_calls.py"
+    script.write_text("""
+import sys
+sys.path[:0] = [%r, %r]
+import numpy as np, torch
+import conftest, test_moe_gpu as t
+smb = conftest.load_package()
+for tokens, top_k, groups in [(84, 8, 512), (81, 8, 512), (116, 8, 384), (36, 8, 1024), (48, 8, 768), (128, 8, 351), (2500, 8, 351)]:
+    ids = np.random.default_rng(groups).integers(-1, groups, size=(tokens, top_k)).astype(np.int32)
+    cap, offsets, rows, slots, _ = t._dispatch(smb, torch, ids, groups)
+    want = t._dispatch_plain(ids, groups, 1, cap)
+    for got, ref in zip((offsets, rows, slots), want):
+        np.testing.assert_array_equal(got.cpu().numpy(), ref)
+print("all equal")
+""" % (str(ROOT), str(ROOT / "tests")))
+    run = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "all equal" in run.stdout, run.stdout + run.stderr
