@@ -187,6 +187,10 @@ struct Top2 {
   __device__ __forceinline__ S value(bool top2) const {
     return top2 && second > S(-INFINITY) ? best + second : best;
   }
+  // What the value is rounded by: its two scores may have opposite signs.
+  __device__ __forceinline__ S size(bool top2) const {
+    return top2 && second > S(-INFINITY) ? fabs(best) + fabs(second) : fabs(best);
+  }
 };
 
 __device__ __forceinline__ float key_score(uint32_t k) { return k > kClosedKey ? key_value(k) : -INFINITY; }
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
     if (by_group) {
       Top2<float> best = {-INFINITY, -INFINITY};
       const bool top2 = (p.flags & SMB_ROUTE_GROUP_TOP2) != 0;
-      float value = -INFINITY;   // lane g of the segment: value of group g
+      float value = -INFINITY, size = 0.0f;   // lane g of the segment: value of group g, and its scores' magnitude
       const int lanes = p.group_lanes;
       if (lanes != 0) {
         // A group has 2^n lanes of its own: join them by shuffles.  Keys of scores are sorted already.
@@ -508,6 +512,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
           best.join(o);
         }
         value = __shfl_sync(kFull, best.value(top2), sl * lanes, L);
+        size = top2 && by_score ? __shfl_sync(kFull, best.size(true), sl * lanes, L) : fabsf(value);
       } else {
         // A padded copy (a word after every 32) for every token of the warp.
         constexpr int kStride = V * L + V * L / 32 + 1;
@@ -520,6 +525,7 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
           for (int i = 0; i < p.group_size; ++i) best.add(buf[sl * p.group_size + i + ((sl * p.group_size + i) >> 5)]);
         __syncwarp();
         value = best.value(top2);
+        size = best.size(top2);
       }
       const uint32_t gkey = sl < p.n_groups ? order_key(value) : 0u;
       // A group stays open if fewer than top_groups come before it (higher value, or equal and lower index).
@@ -530,12 +536,12 @@ __global__ void __launch_bounds__(kWarps * 32, V <= 8 ? 12 : 6) route_kernel(con
       }
       const bool in = sl < p.n_groups && ahead < p.top_groups;
       uint32_t kept = seg_ballot<L>(in, lane);
-      // Only the border matters: the last group kept against the first left out.
-      const uint32_t last = ~seg_max<L>(in ? ~gkey : 0u);
-      const uint32_t first = seg_max<L>(in ? 0u : gkey);
-      const float v = key_value(last), w = key_value(first);
-      // Sums of up to two scores, each with its rounding and hidden position bits.
-      const bool tie = first > kClosedKey && v - w <= 2.0f * slack + 0x1p-23f * (kPos + 3) * (fabsf(v) + fabsf(w));
+      // Only the border matters: the lowest value that a kept group may have against the highest of one left out.
+      // Values are sums of up to two scores, each with its rounding and hidden position bits.
+      const float reach = slack + 0x1p-23f * (kPos + 3) * fminf(size, FLT_MAX);
+      const float low = -seg_max_float<L>(in ? reach - value : -INFINITY);
+      const float high = seg_max_float<L>(!in && sl < p.n_groups && value > -INFINITY ? value + reach : -INFINITY);
+      const bool tie = high > -INFINITY && high >= low;
       if (__any_sync(kFull, tie)) kept = groups_in_fp64<V, L, kBf16, kSpread>(p, row, valid, buf_all[warp], lane);
       if (lanes != 0) {
         // A closed lane never wins, so its head alone keeps it out.

@@ -706,6 +706,25 @@ def test_rows_on_another_stream(smb, cuda_device):
     assert bool(((y.double() - x.double()).abs() <= 2.0 ** -8 * x.double().abs() + 64 * U * x.double().abs()).all())
 
 
+@pytest.mark.parametrize("case", [(500, 256, 8, 8, 4), (300, 160, 6, 8, 3), (200, 510, 8, 17, 6), (400, 64, 4, 4, 2)], ids=str)
+@pytest.mark.parametrize("sigmoid", [False, True])
+@pytest.mark.parametrize("size", [1.0, 16.0, 64.0])
+def test_route_group_sums_that_cancel(smb, cuda_device, case, sigmoid, size):
+    """Biases of either sign: a group's two best scores are +-size + p and all but cancel, so their sum is far smaller
+    than what its rounding goes by.  The 64-bit sums differ by 1e-5 and are off by 2^-45."""
+    torch = _torch()
+    tokens, experts, top_k, n_groups, top_groups = case
+    rng = np.random.default_rng(int(size) + experts + sigmoid)
+    l = _logits(rng, tokens, experts, 1e-3 if sigmoid else 1e-2)
+    bias = np.full(experts, -size, dtype=np.float32)
+    per = experts // n_groups
+    bias[np.arange(n_groups) * per + rng.integers(0, per, n_groups)] = size
+    flags = smb.capi.ROUTE_GROUP_TOP2 | (smb.capi.ROUTE_SIGMOID if sigmoid else 0)
+    _, ids, _ = _route(smb, torch, l, smb.capi.DTYPE_F32, top_k, bias, n_groups, top_groups, flags)
+    want, _ = _route_plain(l.astype(np.float64), bias, top_k, n_groups, top_groups, sigmoid, False, True, 1.0)
+    np.testing.assert_array_equal(ids.cpu().numpy(), want)
+
+
 def test_dispatch_histograms_just_below_the_default_shared_memory(tmp_path):
     """Histograms of 47.9 to 48 KB, in a process whose first calls they are: nothing has raised the kernel's limit
     before.  The last case sorts on a cluster."""
