@@ -26,23 +26,47 @@ _GATHER_I8 = struct.Struct("@11q").pack
 _COMBINE = struct.Struct("@11q").pack
 _COMBINE_BACKWARD = struct.Struct("@14q").pack
 
+# Element types by name; 16-bit integers hold bf16 bit patterns.
+_KINDS = {"float32": capi.DTYPE_F32, "bfloat16": capi.DTYPE_BF16, "uint16": capi.DTYPE_BF16, "int16": capi.DTYPE_BF16}
+_kind_of_type: dict = {}
 
-def route_device(logits, ids, weights, tokens: int, experts: int, top_k: int, dtype: int = capi.DTYPE_F32, bias=None,
+
+def _kind(x, dtype: int | None) -> int:
+    """DTYPE_* of a buffer: its own type, which has to agree with `dtype`; for a raw address `dtype`, or fp32."""
+    own = getattr(x, "dtype", None)
+    if own is None:
+        return capi.DTYPE_F32 if dtype is None else dtype
+    try:
+        kind = _kind_of_type[own]
+    except KeyError:
+        kind = _kind_of_type[own] = _KINDS.get(str(own).removeprefix("torch."))
+    if kind is None:
+        raise ValueError(f"logits and their gradient are fp32 or bf16, not {own}")
+    if dtype is not None and dtype != kind:
+        raise ValueError(f"dtype {dtype} does not agree with a buffer of {own}")
+    return kind
+
+
+def route_device(logits, ids, weights, tokens: int, experts: int, top_k: int, dtype: int | None = None, bias=None,
                  n_groups: int = 1, top_groups: int = 1, flags: int = 0, scale: float = 1.0, ld: int | None = None,
                  stream=None) -> None:
     """ids [tokens, top_k] int32 and weights [tokens, top_k] fp32 from logits [tokens, experts]; closed
-    slots hold id -1, weight 0.  `flags`: capi.ROUTE_*."""
+    slots hold id -1, weight 0.  `flags`: capi.ROUTE_*.  The logits are fp32 or bf16; `dtype` (capi.DTYPE_*) says
+    which where a raw address does not (default fp32), and has to agree with the buffer where it does."""
     capi.call_words(capi.CALL_MOE_ROUTE, _ROUTE(
-        _addr(logits), dtype, experts if ld is None else ld, _addr(bias), tokens, experts, top_k, n_groups, top_groups,
+        _addr(logits), _kind(logits, dtype), experts if ld is None else ld, _addr(bias), tokens, experts, top_k, n_groups, top_groups,
         flags, scale, _addr(ids), _addr(weights), _stream_ptr(stream)), 14)
 
 
 def route_backward_device(logits, ids, grad_weights, grad_logits, tokens: int, experts: int, top_k: int,
-                          dtype: int = capi.DTYPE_F32, flags: int = 0, scale: float = 1.0, ld: int | None = None,
+                          dtype: int | None = None, flags: int = 0, scale: float = 1.0, ld: int | None = None,
                           ld_grad: int | None = None, stream=None) -> None:
-    """grad_logits [tokens, experts] for the ids of the forward pass."""
+    """grad_logits [tokens, experts], in the logits' type, for the ids of the forward pass.  `dtype` as above."""
+    kind = _kind(logits, dtype)
+    if getattr(grad_logits, "dtype", None) is not None:
+        _kind(grad_logits, kind)
     capi.call_words(capi.CALL_MOE_ROUTE_BACKWARD, _ROUTE_BACKWARD(
-        _addr(logits), dtype, experts if ld is None else ld, _addr(ids), _addr(grad_weights), tokens, experts, top_k, flags,
+        _addr(logits), kind, experts if ld is None else ld, _addr(ids), _addr(grad_weights), tokens, experts, top_k, flags,
         scale, _addr(grad_logits), experts if ld_grad is None else ld_grad, _stream_ptr(stream)), 13)
 
 

@@ -246,3 +246,37 @@ def test_calls_by_words_refusals(smb):
     _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, None, 8), "no words")
     _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, b"\0" * 120, 15), "no words")
     _refused(smb, words(smb.capi.CALL_QUANTIZE_I8, b"\0" * 8, -1), "no words")
+
+
+def _words_of(smb, monkeypatch, fn, *args, **kw):
+    """The argument words that a wrapper would hand to the library."""
+    seen = []
+    monkeypatch.setattr(smb.capi, "call_words", lambda call, words, count: seen.append(np.frombuffer(words, np.int64)))
+    fn(*args, **kw)
+    return seen[-1]
+
+
+def test_route_takes_the_type_of_its_buffers(smb, monkeypatch):
+    """Without a word about the type a bf16 buffer is read as one, not four bytes an element to past its end."""
+    torch = pytest.importorskip("torch")
+    f32, bf16 = torch.zeros(2, 8), torch.zeros(2, 8, dtype=torch.bfloat16)
+    ids, w = torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2, 2)
+    m, c = smb.moe, smb.capi
+    for x, kind in ((f32, c.DTYPE_F32), (bf16, c.DTYPE_BF16), (bf16.view(torch.int16), c.DTYPE_BF16), (f32.numpy(), c.DTYPE_F32),
+                    (np.zeros((2, 8), np.uint16), c.DTYPE_BF16), (0x10000, c.DTYPE_F32)):
+        assert _words_of(smb, monkeypatch, m.route_device, x, ids, w, 2, 8, 2)[1] == kind
+        assert _words_of(smb, monkeypatch, m.route_device, x, ids, w, 2, 8, 2, dtype=kind)[1] == kind
+        assert _words_of(smb, monkeypatch, m.route_backward_device, x, ids, w, x, 2, 8, 2)[1] == kind
+    assert _words_of(smb, monkeypatch, m.route_device, 0x10000, ids, w, 2, 8, 2, dtype=c.DTYPE_BF16)[1] == c.DTYPE_BF16
+    for x, kind in ((f32, c.DTYPE_BF16), (bf16, c.DTYPE_F32), (f32, 7)):
+        with pytest.raises(ValueError, match="agree"):
+            m.route_device(x, ids, w, 2, 8, 2, dtype=kind)
+        with pytest.raises(ValueError, match="agree"):
+            m.route_backward_device(x, ids, w, x, 2, 8, 2, dtype=kind)
+    with pytest.raises(ValueError, match="agree"):
+        m.route_backward_device(bf16, ids, w, f32, 2, 8, 2)
+    for t in (torch.float16, torch.float64, torch.int32):
+        with pytest.raises(ValueError, match="fp32 or bf16"):
+            m.route_device(torch.zeros(2, 8, dtype=t), ids, w, 2, 8, 2)
+        with pytest.raises(ValueError, match="fp32 or bf16"):
+            m.route_backward_device(f32, ids, w, torch.zeros(2, 8, dtype=t), 2, 8, 2)

@@ -747,3 +747,18 @@ print("all equal")
 """ % (str(ROOT), str(ROOT / "tests")))
     run = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "all equal" in run.stdout, run.stdout + run.stderr
+
+
+def test_route_of_bf16_without_a_word_about_the_type(smb, cuda_device):
+    torch = _torch()
+    c = smb.capi
+    l = torch.from_numpy(_logits(np.random.default_rng(3), 50, 64)).cuda().bfloat16()
+    out = []
+    for dtype in (None, c.DTYPE_BF16):
+        ids, w = torch.zeros(50, 4, device="cuda", dtype=torch.int32), torch.zeros(50, 4, device="cuda")
+        grad = torch.zeros_like(l)
+        smb.moe.route_device(l, ids, w, 50, 64, 4, dtype=dtype)
+        smb.moe.route_backward_device(l, ids, w, grad, 50, 64, 4, dtype=dtype)
+        out.append((ids, w, grad))
+    assert all(torch.equal(a, b) for a, b in zip(*out))
+    assert torch.equal(out[0][0].long(), l.float().sort(descending=True, stable=True).indices[:, :4])
