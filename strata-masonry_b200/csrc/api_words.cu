@@ -1,6 +1,7 @@
 // The stream-ordered calls around the grouped products with their arguments as 64-bit words, for bindings that
 // pay for every argument they convert.  A decode step makes several of these calls, each for a kernel of two
 // microseconds: from Python a call of fourteen converted arguments takes 4 us, one of a packed string 1.1.
+#include <cmath>
 #include <cstring>
 #include <tuple>
 #include <type_traits>
@@ -21,6 +22,7 @@ bool take(int64_t w, T& out) {
     double v;
     memcpy(&v, &w, 8);
     out = static_cast<T>(v);
+    return std::isinf(out) == std::isinf(v);
   } else {
     out = static_cast<T>(w);
     return static_cast<int64_t>(out) == w;

@@ -280,3 +280,13 @@ def test_route_takes_the_type_of_its_buffers(smb, monkeypatch):
             m.route_device(torch.zeros(2, 8, dtype=t), ids, w, 2, 8, 2)
         with pytest.raises(ValueError, match="fp32 or bf16"):
             m.route_backward_device(f32, ids, w, torch.zeros(2, 8, dtype=t), 2, 8, 2)
+
+
+def test_calls_by_words_refuse_a_scale_beyond_fp32(smb):
+    def route(scale):     # no tokens: valid and without effect
+        smb.moe.route_device(0x10000, 0x10000, 0x10000, 0, 8, 2, scale=scale)
+    for scale in (1.0, 0.1, 3.4e38, -3.4e38, 1e-60, float("inf"), float("nan")):
+        route(scale)
+    for scale in (1e39, -1e300):
+        with pytest.raises(smb.SmbError, match="does not fit"):
+            route(scale)
