@@ -762,3 +762,54 @@ def test_route_of_bf16_without_a_word_about_the_type(smb, cuda_device):
         out.append((ids, w, grad))
     assert all(torch.equal(a, b) for a, b in zip(*out))
     assert torch.equal(out[0][0].long(), l.float().sort(descending=True, stable=True).indices[:, :4])
+
+
+def test_router_feeds_the_fp4_grouped_plan(smb, cuda_device):
+    """Routed rows, quantised to FP4 in groups of whole 256-row tiles, against a dense FP4 product of all tokens with
+    every expert: the same codes and scales, so the same bits in every row that a slot names."""
+    torch = _torch()
+    tokens, experts, top_k, width, n = 300, 5, 2, 256, 384
+    lib, u8 = smb.capi.lib(), dict(device="cuda", dtype=torch.uint8)
+
+    def quantised(rows):
+        codes = torch.empty(rows.shape[0], width // 2, **u8)
+        scales = torch.empty(smb.gemm.sf_packed_bytes(rows.shape[0], width), **u8)
+        smb.capi.check(lib.smb_quantize_mx_bf16_device(rows.data_ptr(), width, codes.data_ptr(), width // 2, scales.data_ptr(),
+                                                       None, rows.shape[0], width, None))
+        return codes, scales
+
+    logits = torch.randn(tokens, experts, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
+    logits[7] = float("-inf")           # a padding token goes nowhere
+    ids = torch.zeros(tokens, top_k, device="cuda", dtype=torch.int32)
+    w = torch.zeros(tokens, top_k, device="cuda")
+    smb.moe.route_device(logits, ids, w, tokens, experts, top_k, flags=smb.capi.ROUTE_RENORM)
+    cap, offsets, row, slot, tiles = _dispatch(smb, torch, ids.cpu().numpy(), experts, 256, 0, True)
+    x, weights = _bf16(torch, tokens, width, seed=1), _bf16(torch, experts * n, width, seed=2)
+    a = torch.zeros(cap, width, device="cuda", dtype=torch.bfloat16)
+    smb.moe.gather_bf16_device(x, row, a, tokens, top_k, width, cap)
+    qa, qb, qx = quantised(a), quantised(weights), quantised(x)
+    d = torch.zeros(cap, n, device="cuda", dtype=torch.bfloat16)
+    plan = smb.gemm.Fp4Plan.grouped(*qa, *qb, d, cap, n, width, experts, tiles)
+    plan.run()
+    plan.check()
+    y = torch.zeros(tokens, n, device="cuda", dtype=torch.bfloat16)
+    smb.moe.combine_device(d, row, w, y, tokens, top_k, n, cap)
+    dense = []
+    for e in range(experts):
+        qe, out = quantised(weights[e * n:(e + 1) * n].contiguous()), torch.zeros(tokens, n, device="cuda", dtype=torch.bfloat16)
+        one = smb.gemm.Fp4Plan(*qx, *qe, out, tokens, n, width)
+        one.run()
+        one.check()
+        dense.append(out)
+    dense = torch.stack(dense)
+    ref, size = torch.zeros(tokens, n, device="cuda", dtype=torch.float64), 0.0
+    for j in range(top_k):
+        live = ids[:, j] >= 0
+        assert bool((live == (row[:, j] >= 0)).all()) and int((~live).sum()) == 1
+        part = dense[ids[live, j].long(), live.nonzero()[:, 0]]
+        assert torch.equal(d[row[live, j].long()], part)
+        ref[live] += part.double() * w[live, j:j + 1].double()
+        size = size + (dense.abs().amax(0).double() * w[:, j:j + 1].double())
+    # Two fused multiply-adds and one rounding to bf16.
+    assert bool(((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 4 * U * size).all())
+    assert not bool(y[7].any())
