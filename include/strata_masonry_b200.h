@@ -467,8 +467,9 @@ int smb_i8_plan_create_bf16_activations(smb_i8_plan** plan, const void* x_bf16, 
 /* Grouped (mixture-of-experts) form with the row offsets in DEVICE memory, as smb_moe_dispatch_device
  * leaves them: group g owns rows [offsets[g], offsets[g + 1]) of A, sa and D and the N rows
  * [g N, (g + 1) N) of B and sb.  `offsets` (groups + 1 ints, not decreasing) is read by every run, so
- * one plan, captured once, serves every batch; max_rows bounds offsets[groups] (rows beyond it are
- * ignored) and sizes A, sa and D.  Rows outside the groups are not written.  At most 512 groups and
+ * one plan, captured once, serves every batch; the plan chooses its kernel by max_rows / groups, so a plan with
+ * room for a prompt batch runs 256-row tiles on a decode batch too (same bits, other speed: a plan of its own
+ * is faster).  max_rows bounds offsets[groups] (rows beyond it are ignored) and sizes A, sa and D.  Rows outside the groups are not written.  At most 512 groups and
  * 2^23 rows. */
 int smb_i8_grouped_plan_create(smb_i8_plan** plan, const void* a, const float* sa, const void* b_stacked,
                                const float* sb_stacked, void* d, int max_rows, int N, int K, int64_t lda,
@@ -502,7 +503,7 @@ int smb_dense_gemm_i8_host(const int8_t* a, const float* sa, const int8_t* b, co
 #define SMB_ROUTE_GROUP_TOP2 4u   /* a group is valued by the sum of its two best scores, else by its best */
 /* logits [tokens, experts] (fp32 or bf16, pitch ld) -> ids [tokens, top_k] and weights [tokens, top_k],
  * best expert first, ties to the lowest index.  Compared are p + bias (bias: [experts] fp32 or NULL; it
- * takes no part in the weights), without a bias the logits.  With top_groups < n_groups only experts of
+ * takes no part in the weights), as fp64 tells them apart, without a bias the logits.  With top_groups < n_groups only experts of
  * the top_groups best of n_groups equal runs of experts can be chosen.  weight = scale * p, or with
  * RENORM scale * p / sum.  ids and weights are contiguous.  Experts whose logit is -inf or NaN (or bias -inf) are closed; where fewer
  * than top_k are open the remaining slots hold id -1 and weight 0 (so a padding row of -inf routes

@@ -1,15 +1,15 @@
 // int8 GEMM for few rows per weight matrix (decode batches, experts with a handful of tokens): bound by
-// reading B once.  Same result, bit for bit, as gemm_i8.cu.  Measured: 16 x 28672 x 8192 with its quantiser 38 us
-// (6.2 TB/s), 128 experts x 256 rows (1536 x 2048 each, gated) 63 us (6.4 TB/s), DRAM reads the operands once
-// (ncu: 235.2 and 404.0 MB).
+// reading B once.  Same result, bit for bit, as gemm_i8.cu.  Measured in a CUDA graph: 16 x 28672 x 8192 with its
+// quantiser 38 us (6.1 TB/s), 128 experts x 256 rows (1536 x 2048 each, gated) 63 us (6.4 TB/s), DRAM reads the
+// operands once (ncu: 235.2 and 404.0 MB).
 //
 // The operands swap roles: 128 rows of B (output channels) fill the rows of a 1-CTA tcgen05.mma and up
 // to 128 rows of A (tokens) its columns, so the instruction does no more work than the tokens need and a
 // stage is mostly weights.  Accumulator lane = channel, column = token.
 //
-// One CTA per SM walks the (row chunk, channel tile) pairs; warp 0 loads (TMA), warp 1 issues the MMAs,
-// warps 2-9 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs cuts the K loop of a
-// pair and adds its int32 partial sums through distributed shared memory: the sums are exact, so their
+// Two CTAs per SM walk the (row chunk, channel tile) pairs; warp 0 loads (TMA), warp 1 issues the MMAs,
+// warps 2-9 drain.  Where there are fewer pairs than SMs, a cluster of up to 8 CTAs for every pair cuts the K loop of
+// the pair and adds its int32 partial sums through distributed shared memory: the sums are exact, so their
 // order does not matter, and there is neither workspace nor atomic.
 //
 // Up to 4 bf16 tokens are quantised in the kernel itself: every CTA finds the scales of all rows (4 x K

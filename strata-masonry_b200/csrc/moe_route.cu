@@ -12,7 +12,8 @@
 //
 // Scores are fp32.  Where two neighbours in the order (or the last chosen and the first left out) lie
 // closer together than the fp32 error of p, fp64 scores of the experts in question decide, so the ids
-// are those of the exact scores whatever exp rounds to.  Choices on bf16 logits need no such care.
+// are those of fp64 scores whatever fp32 makes of them.  (What fp64 cannot tell apart ties: softmax values more than
+// 700 below the largest logit, sigmoid values above 37.)  Choices on bf16 logits need no such care.
 //
 // Renormalised weights are formed from exponentials relative to the largest chosen one, so tiny
 // probabilities do not underflow before they are divided.

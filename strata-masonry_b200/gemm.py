@@ -486,7 +486,8 @@ class I8Plan:
     def grouped(cls, a, sa, b_stacked, sb_stacked, d, max_rows: int, n: int, k: int, groups: int, offsets,
                 lda: int | None = None, ldb: int | None = None, ldd: int | None = None, flags: int = 0):
         """Grouped (mixture-of-experts) form; `offsets` is a device int32 array of groups + 1 row offsets that
-        every run reads (moe.dispatch_device writes it)."""
+        every run reads (moe.dispatch_device writes it).  The kernel is chosen by max_rows / groups, whatever a
+        batch holds: keep a plan of its own for decode batches."""
         self = cls.__new__(cls)
         self._lib = capi.lib()
         self._h = C.c_void_p()
