@@ -26,25 +26,37 @@ _GATHER_I8 = struct.Struct("@11q").pack
 _COMBINE = struct.Struct("@11q").pack
 _COMBINE_BACKWARD = struct.Struct("@14q").pack
 
-# Element types by name; 16-bit integers hold bf16 bit patterns.
-_KINDS = {"float32": capi.DTYPE_F32, "bfloat16": capi.DTYPE_BF16, "uint16": capi.DTYPE_BF16, "int16": capi.DTYPE_BF16}
-_kind_of_type: dict = {}
+# Element types by name: those that say what a buffer holds, and integers, which may be the bits of anything (16-bit
+# ones are taken for bf16 unless the caller says otherwise).
+_FLOATS = {"float32": capi.DTYPE_F32, "bfloat16": capi.DTYPE_BF16}
+_BITS = {"uint16": capi.DTYPE_BF16, "int16": capi.DTYPE_BF16}
+_kind_of_type: dict = {}   # type -> (DTYPE_*, whether the type itself says so); DTYPE_* None: no logits
+
+
+def _kind_of(own):
+    name = str(own).removeprefix("torch.")
+    if "float" in name or "complex" in name:
+        return _FLOATS.get(name), True
+    return _BITS.get(name, capi.DTYPE_F32), False
 
 
 def _kind(x, dtype: int | None) -> int:
-    """DTYPE_* of a buffer: its own type, which has to agree with `dtype`; for a raw address `dtype`, or fp32."""
+    """DTYPE_* of a buffer: its own type where that is a floating one, which has to agree with `dtype`; else (integers,
+    raw addresses) `dtype`, or fp32."""
     own = getattr(x, "dtype", None)
     if own is None:
         return capi.DTYPE_F32 if dtype is None else dtype
     try:
-        kind = _kind_of_type[own]
+        kind, certain = _kind_of_type[own]
     except KeyError:
-        kind = _kind_of_type[own] = _KINDS.get(str(own).removeprefix("torch."))
+        kind, certain = _kind_of_type[own] = _kind_of(own)
     if kind is None:
         raise ValueError(f"logits and their gradient are fp32 or bf16, not {own}")
-    if dtype is not None and dtype != kind:
+    if dtype is None:
+        return kind
+    if certain and dtype != kind:
         raise ValueError(f"dtype {dtype} does not agree with a buffer of {own}")
-    return kind
+    return dtype
 
 
 def route_device(logits, ids, weights, tokens: int, experts: int, top_k: int, dtype: int | None = None, bias=None,

@@ -267,7 +267,12 @@ def test_route_takes_the_type_of_its_buffers(smb, monkeypatch):
         assert _words_of(smb, monkeypatch, m.route_device, x, ids, w, 2, 8, 2)[1] == kind
         assert _words_of(smb, monkeypatch, m.route_device, x, ids, w, 2, 8, 2, dtype=kind)[1] == kind
         assert _words_of(smb, monkeypatch, m.route_backward_device, x, ids, w, x, 2, 8, 2)[1] == kind
-    assert _words_of(smb, monkeypatch, m.route_device, 0x10000, ids, w, 2, 8, 2, dtype=c.DTYPE_BF16)[1] == c.DTYPE_BF16
+    # Integers hold the bits of whatever the caller says, as raw addresses do.
+    for x in (0x10000, torch.zeros(64, dtype=torch.uint8), f32.view(torch.int32), bf16.view(torch.int16)):
+        for kind in (c.DTYPE_F32, c.DTYPE_BF16):
+            assert _words_of(smb, monkeypatch, m.route_device, x, ids, w, 2, 8, 2, dtype=kind)[1] == kind
+            assert _words_of(smb, monkeypatch, m.route_backward_device, x, ids, w, x, 2, 8, 2, dtype=kind)[1] == kind
+    assert _words_of(smb, monkeypatch, m.route_device, f32.view(torch.int32), ids, w, 2, 8, 2)[1] == c.DTYPE_F32
     for x, kind in ((f32, c.DTYPE_BF16), (bf16, c.DTYPE_F32), (f32, 7)):
         with pytest.raises(ValueError, match="agree"):
             m.route_device(x, ids, w, 2, 8, 2, dtype=kind)
@@ -275,7 +280,7 @@ def test_route_takes_the_type_of_its_buffers(smb, monkeypatch):
             m.route_backward_device(x, ids, w, x, 2, 8, 2, dtype=kind)
     with pytest.raises(ValueError, match="agree"):
         m.route_backward_device(bf16, ids, w, f32, 2, 8, 2)
-    for t in (torch.float16, torch.float64, torch.int32):
+    for t in (torch.float16, torch.float64, torch.complex64):
         with pytest.raises(ValueError, match="fp32 or bf16"):
             m.route_device(torch.zeros(2, 8, dtype=t), ids, w, 2, 8, 2)
         with pytest.raises(ValueError, match="fp32 or bf16"):
