@@ -64,10 +64,10 @@ def route_device(logits, ids, weights, tokens: int, experts: int, top_k: int, dt
                  stream=None) -> None:
     """ids [tokens, top_k] int32 and weights [tokens, top_k] fp32 from logits [tokens, experts]; closed
     slots hold id -1, weight 0.  `flags`: capi.ROUTE_*.  The logits are fp32 or bf16; `dtype` (capi.DTYPE_*) says
-    which where a raw address does not (default fp32), and has to agree with the buffer where it does."""
+    which where the buffer does not (a raw address, integers; default fp32), and has to agree with it where it does."""
     capi.call_words(capi.CALL_MOE_ROUTE, _ROUTE(
-        _addr(logits), _kind(logits, dtype), experts if ld is None else ld, _addr(bias), tokens, experts, top_k, n_groups, top_groups,
-        flags, scale, _addr(ids), _addr(weights), _stream_ptr(stream)), 14)
+        _addr(logits), _kind(logits, dtype), experts if ld is None else ld, _addr(bias), tokens, experts, top_k, n_groups,
+        top_groups, flags, scale, _addr(ids), _addr(weights), _stream_ptr(stream)), 14)
 
 
 def route_backward_device(logits, ids, grad_weights, grad_logits, tokens: int, experts: int, top_k: int,
